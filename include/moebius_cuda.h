@@ -48,6 +48,15 @@ extern "C" {
 /* Weight storage precision (reference Param, src/engine/param.rs:14-17). */
 #define MBX_DTYPE_F32 0
 #define MBX_DTYPE_F16 1
+/* Storage of the image-token attention operators only (no weights). */
+#define MBX_DTYPE_BF16 2
+
+/* Channels that a rotation turns together: (2i, 2i + 1), or (i, i + D/2) of a section of D channels. */
+#define MBX_ROPE_ADJACENT 0
+#define MBX_ROPE_HALVES   1
+
+/* Query rows that share one selection of key blocks. */
+#define MBX_ATTENTION_BLOCK_Q 128
 
 /* Depthwise epilogues (reference depthwise::Epilogue, src/engine/depthwise.rs:23-28). */
 #define MBX_EPILOGUE_NONE     0
@@ -267,6 +276,74 @@ int32_t mbx_gemm(mbx_ctx *ctx, float *c, const float *a, int64_t m, int64_t k, c
 /* out = x * mul + add over len floats (out may equal x). Reference: the decoder's
  * latent unscale and (x + 1) / 2, src/vae/decoder.rs:81,97. */
 int32_t mbx_scale_add(mbx_ctx *ctx, const float *x, int64_t len, float mul, float add, float *out);
+
+/* ---------------------------------------------------------------- image-token attention
+ * Attention of image and video tokens over selected key blocks, between two
+ * projections (mbx_conv1x1): mbx_qkv_norm_rope turns the packed projection into
+ * normalised, rotated heads, mbx_block_select chooses key blocks for every 128
+ * query rows, mbx_block_attention attends to them. No reference counterpart: the
+ * reference's only attention is the dense one of src/vae/mod.rs:240-270.
+ *
+ * Head tensors are token-major, [n][tokens][heads][dim], in float32, float16 or
+ * bfloat16 (MBX_DTYPE_*); sums, statistics and exponentials are float32 or wider.
+ * Query head h reads key/value head h / (heads / kv_heads); kv_heads divides
+ * heads. A *_stride is the number of elements between two tokens, at least the
+ * row's own length, so a part of a packed row serves in place; item i starts at
+ * i * tokens * stride. Pointers are 16-byte aligned, rows a multiple of 16 bytes
+ * apart, dim a multiple of 8. The results are deterministic. */
+
+/* Splits the rows of a packed projection x [n][tokens][x_stride], each
+ * [q heads | k kv_heads | v kv_heads] x dim, into q [n][tokens][heads][dim] and
+ * k, v [n][tokens][kv_heads][dim] (dense, in out_dtype):
+ *  - with norm != 0, every q and k head is first y = x * gamma / sqrt(mean(x^2) + eps),
+ *    gamma = q_gamma or k_gamma [dim] (NULL: ones);
+ *  - with positions != NULL, axis a (time, height, width) then turns its section of
+ *    axis_dims[a] channels (even, 0 leaves the axis out; sections lie one behind the other
+ *    from channel 0, channels behind the last are not rotated): pair i by the angle
+ *    positions[item][token][a] * theta^(-2i / axis_dims[a]), (y0, y1) ->
+ *    (y0 cos - y1 sin, y1 cos + y0 sin), in the pairing MBX_ROPE_*. positions is float32
+ *    [position_items][tokens][3], position_items = n or 1 (shared); angles are reduced in
+ *    float64, so far positions keep their precision;
+ *  - v is only converted. v may be NULL (the row's v part need not exist then); k may be NULL
+ *    only with kv_heads = 0, q only with heads = 0.
+ * dim <= 256. x_dtype f32 goes to any out_dtype; f16 and bf16 stay as they are. Outputs must
+ * not overlap x. Values are rounded once, from float32 to out_dtype. */
+int32_t mbx_qkv_norm_rope(mbx_ctx *ctx, const void *x, int32_t x_dtype, int64_t n, int64_t tokens, int64_t x_stride,
+                          int64_t heads, int64_t kv_heads, int64_t dim, int32_t norm, const float *q_gamma,
+                          const float *k_gamma, float eps, const float *positions, int64_t position_items,
+                          const int64_t axis_dims[3], double theta, int32_t pairing, void *q, void *k, void *v,
+                          int32_t out_dtype);
+
+/* For each item, head and block of MBX_ATTENTION_BLOCK_Q query rows (the last one may be
+ * shorter), the topk key blocks of block_k tokens (16, 32, 64 or 128; the last may be shorter)
+ * with the highest score, (mean of the block's queries) . (mean of the block's unmasked keys),
+ * a tie going to the lower block: index [n][heads][ceil(nq / 128)][topk] in ascending order,
+ * -1 where fewer blocks have an unmasked key. key_mask [n][nk] bytes, nonzero = may be
+ * attended to (NULL: all); masked keys may hold anything. Means and scores are float64, so the
+ * choice does not hang on the order of a sum; a score of NaN counts as the highest.
+ * workspace: mbx_block_select_workspace bytes of device memory, 256-byte aligned, that no
+ * other call in flight uses. */
+int32_t mbx_block_select_workspace(int64_t n, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t dim,
+                                   int64_t block_k, size_t *bytes);
+int32_t mbx_block_select(mbx_ctx *ctx, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                         int32_t dtype, int64_t n, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
+                         int64_t dim, int64_t block_k, const uint8_t *key_mask, int64_t topk, int32_t *index,
+                         void *workspace, size_t workspace_bytes);
+
+/* out [n][nq][heads][dim] = softmax(scale * q k^T) v over the keys of the blocks that
+ * index [n][heads][ceil(nq / 128)][topk] lists for the row's query block (mbx_block_select's
+ * layout, from there or from the caller) and that key_mask keeps. Entries outside
+ * [0, ceil(nk / block_k)) are skipped; a block listed twice counts twice. A row with no key left
+ * is zero. Masked keys and values may hold anything; the others are finite. dim <= 128; q, k, v
+ * and out have the same dtype. out must not overlap an input. workspace as for mbx_block_select
+ * (the size may be 0, and workspace NULL then). */
+int32_t mbx_block_attention_workspace(int32_t dtype, int64_t n, int64_t nq, int64_t nk, int64_t heads,
+                                      int64_t kv_heads, int64_t dim, int64_t block_k, int64_t topk, size_t *bytes);
+int32_t mbx_block_attention(mbx_ctx *ctx, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                            const void *v, int64_t v_stride, int32_t dtype, int64_t n, int64_t nq, int64_t nk,
+                            int64_t heads, int64_t kv_heads, int64_t dim, int64_t block_k, const uint8_t *key_mask,
+                            const int32_t *index, int64_t topk, float scale, void *out, void *workspace,
+                            size_t workspace_bytes);
 
 /* ---------------------------------------------------------------- lambda layers (UNet) */
 

@@ -22,12 +22,19 @@ context stream and mirrors one reference engine call:
 ``matmul``             gemm::matmul (src/engine/gemm.rs:63-132)
 =====================  ==========================================================
 
+Attention of image and video tokens over selected key blocks (no reference
+counterpart): ``qkv_norm_rope`` splits a packed projection into normalised,
+rotated heads, ``block_select`` chooses key blocks for every 128 query rows and
+``block_attention`` attends to them. These take float32, float16 and bfloat16
+(``bfloat16``: the two bytes as a NumPy field, ``x.view(np.uint16)``).
+
 Import with ``importlib.import_module("moebius-cpu_b200")`` (the directory
 name is not a Python identifier).
 """
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Sequence
 
 import numpy as np
@@ -38,9 +45,15 @@ from .abi import MbxError, check, lib
 __all__ = ["Context", "DeviceTensor", "Param", "MbxError", "abi", "group_norm", "group_norm_affine",
            "group_norm_apply", "layer_norm", "depthwise3x3", "conv1x1", "conv3x3", "conv3x3_output_hw",
            "silu_inplace", "add_inplace", "concat_channels", "bias_temb_add", "matmul", "conv_group_norm_affine",
-           "EPILOGUES"]
+           "EPILOGUES", "PAIRINGS", "bfloat16", "qkv_norm_rope", "block_select", "block_select_workspace",
+           "block_attention", "block_attention_workspace"]
 
 EPILOGUES = {"none": abi.EPILOGUE_NONE, "relu": abi.EPILOGUE_RELU, "glu_silu": abi.EPILOGUE_GLU_SILU}
+PAIRINGS = {"adjacent": abi.ROPE_ADJACENT, "halves": abi.ROPE_HALVES}
+
+#: NumPy has no bfloat16: its sixteen bits as a one-field type.
+bfloat16 = np.dtype([("bfloat16", "<u2")])
+_STORAGE = {np.dtype(np.float32): abi.DTYPE_F32, np.dtype(np.float16): abi.DTYPE_F16, bfloat16: abi.DTYPE_BF16}
 
 
 class Context:
@@ -130,7 +143,7 @@ class DeviceTensor:
         self.ctx = ctx
         self.shape = tuple(shape)
         self.dtype = np.dtype(dtype)
-        self.size = int(np.prod(self.shape)) if self.shape else 1
+        self.size = math.prod(self.shape)
         self.nbytes = self.dtype.itemsize * self.size
         self.owned = ptr is None
         self.ptr = ctx.alloc(self.nbytes) if ptr is None else int(ptr)
@@ -348,6 +361,119 @@ def matmul(a: DeviceTensor, b: DeviceTensor, c: Optional[DeviceTensor] = None,
     c = c or a.ctx.empty((m, n))
     check(lib().mbx_matmul(a.ctx.handle, c.vp, a.vp, m, k, k, 1, b.vp, n, n, 1, int(accumulate)))
     return c
+
+
+def _storage(t: DeviceTensor) -> int:
+    code = _STORAGE.get(t.dtype)
+    if code is None:
+        raise ValueError("expected float32, float16 or bfloat16")
+    return code
+
+
+def _fits(t: Optional[DeviceTensor], shape: tuple, dtype, what: str) -> None:
+    """A tensor of the caller's holds what a kernel reads or writes there."""
+    if t is not None and (t.shape != shape or t.dtype != dtype):
+        raise ValueError(f"{what} must be {dtype} of shape {shape}, not {t.dtype} of {t.shape}")
+
+
+def qkv_norm_rope(x: DeviceTensor, heads: int, kv_heads: int, dim: int, positions: Optional[DeviceTensor] = None,
+                  axis_dims: Sequence[int] = (0, 0, 0), theta: float = 10000.0, pairing: str = "adjacent",
+                  norm: bool = True, q_gamma: Optional[DeviceTensor] = None, k_gamma: Optional[DeviceTensor] = None,
+                  eps: float = 1e-6, dtype=None, out=None):
+    """Splits packed rows x [n, tokens, >= (heads + 2 kv_heads) dim] into q [n, tokens, heads, dim] and k, v [n, tokens,
+    kv_heads, dim] of `dtype` (x's by default), q and k normalised per head and rotated by positions
+    [n or 1, tokens, 3] or [tokens, 3] (time, height, width) in sections of axis_dims channels (mbx_qkv_norm_rope).
+    out = (q, k, v); a v of None is left out, and x's rows need not hold it."""
+    n, tokens, stride = x.shape
+    if out is None:
+        dtype = x.dtype if dtype is None else np.dtype(dtype)
+        out = (x.ctx.empty((n, tokens, heads, dim), dtype), x.ctx.empty((n, tokens, kv_heads, dim), dtype),
+               x.ctx.empty((n, tokens, kv_heads, dim), dtype))
+    q, k, v = out
+    kind = next(t for t in out if t is not None).dtype
+    for t, h, what in ((q, heads, "q"), (k, kv_heads, "k"), (v, kv_heads, "v")):
+        _fits(t, (n, tokens, h, dim), kind, what)
+    for t, what in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+        _fits(t, (dim,), np.float32, what)
+    items = 1
+    if positions is not None:
+        items = positions.shape[0] if len(positions.shape) == 3 else 1
+        _fits(positions, (items,) * (len(positions.shape) - 2) + (tokens, 3), np.float32, "positions")
+    check(lib().mbx_qkv_norm_rope(x.ctx.handle, x.vp, _storage(x), n, tokens, stride, heads, kv_heads, dim, int(norm),
+                                  _vp(q_gamma), _vp(k_gamma), eps, _vp(positions), items,
+                                  (ctypes.c_int64 * 3)(*axis_dims), theta, PAIRINGS[pairing], _vp(q), _vp(k), _vp(v),
+                                  _STORAGE.get(kind, -1)))
+    return out
+
+
+def _heads(q: DeviceTensor, k: DeviceTensor):
+    """(n, nq, nk, heads, kv_heads, dim) of token-major head tensors."""
+    if len(q.shape) != 4 or len(k.shape) != 4 or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError("expected q [n, nq, heads, dim] and k [n, nk, kv_heads, dim]")
+    if q.dtype != k.dtype:
+        raise ValueError("q and k differ in type")
+    return q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3]
+
+
+def _scratch(ctx: Context, nbytes: int) -> DeviceTensor:
+    return ctx.empty((nbytes,), np.uint8)
+
+
+def block_select_workspace(q: DeviceTensor, k: DeviceTensor, block_k: int = 64) -> DeviceTensor:
+    """Scratch for block_select calls of these shapes, one at a time."""
+    need = ctypes.c_size_t()
+    check(lib().mbx_block_select_workspace(*_heads(q, k), block_k, ctypes.byref(need)))
+    return _scratch(q.ctx, need.value)
+
+
+def block_select(q: DeviceTensor, k: DeviceTensor, topk: int, block_k: int = 64,
+                 key_mask: Optional[DeviceTensor] = None, q_stride: Optional[int] = None,
+                 k_stride: Optional[int] = None, workspace: Optional[DeviceTensor] = None,
+                 out: Optional[DeviceTensor] = None) -> DeviceTensor:
+    """The topk best key blocks of every 128 query rows, index [n, heads, ceil(nq / 128), topk] (mbx_block_select).
+    q_stride, k_stride: elements between tokens where the heads are part of wider rows."""
+    n, nq, nk, heads, kv_heads, dim = _heads(q, k)
+    shape = (n, heads, -(-nq // abi.ATTENTION_BLOCK_Q), topk)
+    out = out or q.ctx.empty(shape, np.int32)
+    _fits(out, shape, np.int32, "out")
+    _fits(key_mask, (n, nk), np.uint8, "key_mask")
+    workspace = workspace or block_select_workspace(q, k, block_k)
+    check(lib().mbx_block_select(q.ctx.handle, q.vp, heads * dim if q_stride is None else q_stride, k.vp,
+                                 kv_heads * dim if k_stride is None else k_stride, _storage(q), n, nq, nk, heads,
+                                 kv_heads, dim, block_k, _vp(key_mask), topk, out.vp, workspace.vp, workspace.nbytes))
+    return out
+
+
+def block_attention_workspace(q: DeviceTensor, k: DeviceTensor, index: DeviceTensor,
+                              block_k: int = 64) -> DeviceTensor:
+    """Scratch for block_attention calls of these shapes, one at a time."""
+    need = ctypes.c_size_t()
+    check(lib().mbx_block_attention_workspace(_storage(q), *_heads(q, k), block_k, index.shape[-1],
+                                              ctypes.byref(need)))
+    return _scratch(q.ctx, need.value)
+
+
+def block_attention(q: DeviceTensor, k: DeviceTensor, v: DeviceTensor, index: DeviceTensor, block_k: int = 64,
+                    key_mask: Optional[DeviceTensor] = None, scale: Optional[float] = None,
+                    q_stride: Optional[int] = None, k_stride: Optional[int] = None, v_stride: Optional[int] = None,
+                    workspace: Optional[DeviceTensor] = None, out: Optional[DeviceTensor] = None) -> DeviceTensor:
+    """softmax(scale q k^T) v over the key blocks that index lists for each 128 query rows (mbx_block_attention);
+    scale is 1 / sqrt(dim) by default."""
+    n, nq, nk, heads, kv_heads, dim = _heads(q, k)
+    _fits(v, k.shape, k.dtype, "v")
+    _fits(index, (n, heads, -(-nq // abi.ATTENTION_BLOCK_Q)) + index.shape[-1:], np.int32, "index")
+    _fits(key_mask, (n, nk), np.uint8, "key_mask")
+    out = out or q.ctx.empty(q.shape, q.dtype)
+    _fits(out, q.shape, q.dtype, "out")
+    workspace = workspace or block_attention_workspace(q, k, index, block_k)
+    kv_row = kv_heads * dim
+    check(lib().mbx_block_attention(q.ctx.handle, q.vp, heads * dim if q_stride is None else q_stride, k.vp,
+                                    kv_row if k_stride is None else k_stride, v.vp,
+                                    kv_row if v_stride is None else v_stride, _storage(q), n, nq, nk, heads, kv_heads,
+                                    dim, block_k, _vp(key_mask), index.vp, index.shape[-1],
+                                    1.0 / math.sqrt(dim) if scale is None else scale, out.vp, workspace.vp,
+                                    workspace.nbytes))
+    return out
 
 
 from . import engine, synthetic  # noqa: E402  (engine API; seeded converter-format weights)

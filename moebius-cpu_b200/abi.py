@@ -29,6 +29,12 @@ ERR_TIMEOUT = 9
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_BF16 = 2
+
+ROPE_ADJACENT = 0
+ROPE_HALVES = 1
+
+ATTENTION_BLOCK_Q = 128
 
 EPILOGUE_NONE = 0
 EPILOGUE_RELU = 1
@@ -118,6 +124,14 @@ SIGNATURES = {
     "mbx_gemm": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _vp]),
     "mbx_scale_add": (_i32, [_vp, _vp, _i64, _f32, _f32, _vp]),
     "mbx_conv1x1_fused": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp]),
+    "mbx_qkv_norm_rope": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _f32, _vp, _i64,
+                                 _pi64, _f64, _i32, _vp, _vp, _vp, _i32]),
+    "mbx_block_select_workspace": (_i32, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _psz]),
+    "mbx_block_select": (_i32, [_vp, _vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64,
+                                _vp, _vp, _sz]),
+    "mbx_block_attention_workspace": (_i32, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _psz]),
+    "mbx_block_attention": (_i32, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i64,
+                                   _i64, _vp, _vp, _i64, _f32, _vp, _vp, _sz]),
     "mbx_lambda_content": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
     "mbx_self_lambda_position": (_i32, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp]),
     "mbx_cross_lambda_position": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),

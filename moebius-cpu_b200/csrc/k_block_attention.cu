@@ -1,0 +1,211 @@
+// Softmax attention of query blocks over listed key blocks.
+//
+//   out[b, r, h] = Σ_j p_j v[b, j, h/g] / Σ_j p_j,  p_j = exp(scale · q[b, r, h]·k[b, j, h/g] − m)
+// over the keys j of the blocks that index[b, h, r / 128] lists and that the
+// key mask keeps; a row without any such key is zero.
+//
+// The rows kernel: one pass over the listed keys with a running maximum and sum (f32). A group of
+// lanes holds one key's channels, eight a lane, so a warp works on several keys at a time; every
+// group keeps its own maximum, sum and output for R query rows and the groups and warps are joined
+// at the end. Where there are few rows the listed blocks are split over several CTAs, whose partial
+// (output, maximum, sum) a second kernel joins.
+#include <algorithm>
+
+#include "mbx_device.cuh"
+#include "mbx_internal.h"
+
+namespace mbx {
+namespace {
+
+constexpr int kRowWarps = 4;
+
+struct AttnArgs {
+    const void *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride, nq, nk, topk;
+    int heads, kv_heads, dim, block_k, k_blocks, q_blocks;
+    const uint8_t* mask;   // [n][nk] or null
+    const int32_t* index;  // [n][heads][q_blocks][topk]
+    float scale;           // scale · log2(e): exponentials are 2^x
+    void* out;             // [n][nq][heads][dim]
+    float* part;           // splits > 1: [n][nq][heads][splits][dim + 2], then the joined result goes to out
+    int splits;
+};
+
+// Lanes of a key's group: the power of two that holds dim / 8.
+template <class T, int R>
+__global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const AttnArgs a, int group) {
+    // One slot per (warp, group, row) and then the join: maxima, sums, outputs.
+    extern __shared__ float sh[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int li = lane & (group - 1), gi = lane / group, groups = 32 / group;
+    const int slots = kRowWarps * groups, slot = warp * groups + gi;
+    const bool holds = li * 8 < a.dim;
+    const int tiles = (int)((a.nq + R - 1) / R);
+    const int64_t cta = blockIdx.x / a.splits;
+    const int split = (int)(blockIdx.x - cta * a.splits);
+    const int64_t r0 = cta % tiles * R;
+    const int h = (int)(cta / tiles % a.heads);
+    const int64_t item = cta / tiles / a.heads;
+    const int kh = h / (a.heads / a.kv_heads);
+    // A tile of R rows never straddles two query blocks: R divides 128.
+    const int32_t* list = a.index + ((item * a.heads + h) * a.q_blocks + r0 / MBX_ATTENTION_BLOCK_Q) * a.topk;
+    const T* q = static_cast<const T*>(a.q) + (item * a.nq + r0) * a.q_stride + (int64_t)h * a.dim + li * 8;
+    const T* k = static_cast<const T*>(a.k) + item * a.nk * a.k_stride + (int64_t)kh * a.dim + li * 8;
+    const T* v = static_cast<const T*>(a.v) + item * a.nk * a.v_stride + (int64_t)kh * a.dim + li * 8;
+    const uint8_t* mask = a.mask ? a.mask + item * a.nk : nullptr;
+
+    float qv[R][8], acc[R][8] = {}, m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY, l[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qv[r][i] = 0.0f;
+        if (holds && r0 + r < a.nq) widen8<T>(load_raw8(q + r * a.q_stride), qv[r]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qv[r][i] *= a.scale;
+    }
+
+    const int64_t first = a.topk * split / a.splits, last = a.topk * (split + 1) / a.splits;
+    for (int64_t e = first; e < last; ++e) {
+        const int blk = list[e];
+        if (blk < 0 || blk >= a.k_blocks) continue;
+        const int64_t j0 = (int64_t)blk * a.block_k;
+        const int keys = (int)min((int64_t)a.block_k, a.nk - j0);
+        for (int s = slot; s - gi - warp * groups < keys; s += slots) {  // the same trips in every lane of the block
+            const int64_t j = j0 + s;
+            const bool on = s < keys && (!mask || mask[j]);
+            float kv[8] = {}, vv[8] = {};
+            if (on && holds) {
+                widen8<T>(load_raw8(k + j * a.k_stride), kv);
+                widen8<T>(load_raw8(v + j * a.v_stride), vv);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float d = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d = fmaf(qv[r][i], kv[i], d);
+                for (int o = group >> 1; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+                if (on && d != -INFINITY) {
+                    const float mn = fmaxf(m[r], d);
+                    const float c = exp2f(m[r] - mn), p = exp2f(d - mn);
+                    m[r] = mn;
+                    l[r] = l[r] * c + p;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[r][i] = fmaf(acc[r][i], c, p * vv[i]);
+                }
+            }
+        }
+    }
+
+    float* sm = sh;                  // [slots][R]
+    float* sl = sm + slots * R;      // [slots][R]
+    float* so = sl + slots * R;      // [slots][R][dim]
+    if (li == 0) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) sm[slot * R + r] = m[r], sl[slot * R + r] = l[r];
+    }
+    if (holds) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) so[(slot * R + r) * a.dim + li * 8 + i] = acc[r][i];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < R * a.dim; e += kRowWarps * 32) {
+        const int r = e / a.dim, ch = e - r * a.dim;
+        if (r0 + r >= a.nq) continue;
+        float top = -INFINITY;
+        for (int s = 0; s < slots; ++s) top = fmaxf(top, sm[s * R + r]);
+        float sum = 0.0f, o = 0.0f;
+        for (int s = 0; s < slots; ++s) {
+            const float ms = sm[s * R + r];
+            const float w = ms == -INFINITY ? 0.0f : exp2f(ms - top);
+            sum = fmaf(w, sl[s * R + r], sum);
+            o = fmaf(w, so[(s * R + r) * a.dim + ch], o);
+        }
+        const int64_t row = (item * a.nq + r0 + r) * a.heads + h;
+        if (a.splits == 1) {
+            static_cast<T*>(a.out)[row * a.dim + ch] = (T)(sum == 0.0f ? 0.0f : o / sum);
+        } else {
+            float* p = a.part + (row * a.splits + split) * (a.dim + 2);
+            p[ch] = o;
+            if (ch == 0) p[a.dim] = top, p[a.dim + 1] = sum;
+        }
+    }
+}
+
+// Joins the splits' partial results: one warp per (row, head).
+template <class T>
+__global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, int64_t rows) {
+    const int64_t row = blockIdx.x * 4ll + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const float* p = a.part + row * a.splits * (a.dim + 2);
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, p[s * (a.dim + 2) + a.dim]);
+    for (int ch = threadIdx.x & 31; ch < a.dim; ch += 32) {
+        float sum = 0.0f, o = 0.0f;
+        for (int s = 0; s < a.splits; ++s) {
+            const float* ps = p + s * (a.dim + 2);
+            const float w = ps[a.dim] == -INFINITY ? 0.0f : exp2f(ps[a.dim] - top);
+            sum = fmaf(w, ps[a.dim + 1], sum);
+            o = fmaf(w, ps[ch], o);
+        }
+        static_cast<T*>(a.out)[row * a.dim + ch] = (T)(sum == 0.0f ? 0.0f : o / sum);
+    }
+}
+
+constexpr int kRowsR = 4;
+
+// Splits of the listed blocks: enough CTAs to fill the card twice over (148 SMs), never more than the listed blocks.
+int row_splits(const BlockShape& s, int64_t topk) {
+    const int64_t ctas = s.n * s.heads * ((s.nq + kRowsR - 1) / kRowsR);
+    const int64_t want = (2 * 148 + ctas - 1) / std::max<int64_t>(ctas, 1);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, topk), 64));
+}
+
+template <class T>
+void launch_rows(mbx_ctx* ctx, const AttnArgs& a, int64_t n) {
+    int group = 1;
+    while (group * 8 < a.dim) group *= 2;
+    const int slots = kRowWarps * (32 / group);
+    const size_t smem = sizeof(float) * (size_t)slots * kRowsR * (a.dim + 2);
+    const int64_t ctas = n * a.heads * ((a.nq + kRowsR - 1) / kRowsR) * a.splits;
+    MBX_REQUIRE(ctas < (int64_t(1) << 31), "block_attention: too many query rows");
+    ensure_smem_limit((const void*)attention_rows_kernel<T, kRowsR>, (int)smem, "attention_rows");
+    attention_rows_kernel<T, kRowsR><<<(unsigned)ctas, kRowWarps * 32, smem, ctx->stream>>>(a, group);
+    after_launch(ctx, "attention_rows");
+    if (a.splits > 1) {
+        const int64_t rows = n * a.nq * a.heads;
+        attention_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, ctx->stream>>>(a, rows);
+        after_launch(ctx, "attention_join");
+    }
+}
+
+}  // namespace
+
+size_t block_attention_bytes(const BlockShape& s, int64_t topk) {
+    const int splits = row_splits(s, topk);
+    return splits > 1 ? align256(sizeof(float) * (size_t)(s.n * s.nq * s.heads) * splits * (s.dim + 2)) : 0;
+}
+
+void launch_block_attention(mbx_ctx* ctx, const BlockShape& s, const void* q, int64_t q_stride, const void* k,
+                            int64_t k_stride, const void* v, int64_t v_stride, const uint8_t* key_mask,
+                            const int32_t* index, int64_t topk, float scale, void* out, void* workspace) {
+    AttnArgs a{};
+    a.q = q, a.k = k, a.v = v;
+    a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
+    a.nq = s.nq, a.nk = s.nk, a.topk = topk;
+    a.heads = (int)s.heads, a.kv_heads = (int)s.kv_heads, a.dim = (int)s.dim, a.block_k = (int)s.block_k;
+    a.k_blocks = (int)((s.nk + s.block_k - 1) / s.block_k);
+    a.q_blocks = (int)((s.nq + MBX_ATTENTION_BLOCK_Q - 1) / MBX_ATTENTION_BLOCK_Q);
+    a.mask = key_mask, a.index = index;
+    a.scale = scale * 1.4426950408889634f;  // log2(e)
+    a.out = out;
+    a.part = static_cast<float*>(workspace);
+    a.splits = row_splits(s, topk);
+    if (s.dtype == MBX_DTYPE_F32) return launch_rows<float>(ctx, a, s.n);
+    if (s.dtype == MBX_DTYPE_F16) return launch_rows<__half>(ctx, a, s.n);
+    launch_rows<__nv_bfloat16>(ctx, a, s.n);
+}
+
+}  // namespace mbx

@@ -43,6 +43,54 @@ void require_ptr(const void* p, const char* what) {
     MBX_REQUIRE(p != nullptr, std::string("null pointer: ") + what);
 }
 
+void require_aligned(const void* p, size_t to, const char* what) {
+    require_ptr(p, what);
+    MBX_REQUIRE((uintptr_t)p % to == 0, std::string(what) + " must be " + std::to_string(to) + "-byte aligned");
+}
+
+// The image-token attention operators: storage types, rows and shapes.
+constexpr int64_t kMaxExtent = (int64_t(1) << 31) - 256;  // items or tokens
+
+int storage_size(int32_t dtype) { return dtype == MBX_DTYPE_F32 ? 4 : 2; }
+
+void require_storage(int32_t dtype) {
+    MBX_REQUIRE(dtype == MBX_DTYPE_F32 || dtype == MBX_DTYPE_F16 || dtype == MBX_DTYPE_BF16,
+                "dtype must be MBX_DTYPE_F32, MBX_DTYPE_F16 or MBX_DTYPE_BF16");
+}
+
+// A row of `row` elements every `stride`, read in 16-byte pieces (a null p is the caller's to refuse).
+void require_rows(const void* p, int64_t stride, int64_t row, int32_t dtype, const char* what) {
+    MBX_REQUIRE(stride >= row && stride < (int64_t(1) << 31), std::string(what) + ": stride shorter than a row");
+    MBX_REQUIRE(stride * storage_size(dtype) % 16 == 0, std::string(what) + ": rows must be 16 bytes apart");
+    MBX_REQUIRE((uintptr_t)p % 16 == 0, std::string(what) + " must be 16-byte aligned");
+}
+
+mbx::BlockShape block_shape(int32_t dtype, int64_t n, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
+                            int64_t dim, int64_t block_k, int64_t max_dim) {
+    require_storage(dtype);
+    MBX_REQUIRE(n >= 0 && nq >= 0 && nk >= 0 && nq < kMaxExtent && nk < kMaxExtent, "bad shape");
+    MBX_REQUIRE(heads > 0 && kv_heads > 0 && heads <= 65535 && heads % kv_heads == 0,
+                "heads must be a multiple of kv_heads");
+    MBX_REQUIRE(n <= 65535 && n * heads <= 65535, "n * heads must be at most 65535");
+    MBX_REQUIRE(dim > 0 && dim <= max_dim && dim % 8 == 0,
+                "dim must be a multiple of 8, at most " + std::to_string(max_dim));
+    MBX_REQUIRE(block_k == 16 || block_k == 32 || block_k == 64 || block_k == 128,
+                "block_k must be 16, 32, 64 or 128");
+    return mbx::BlockShape{dtype, n, nq, nk, heads, kv_heads, dim, block_k};
+}
+
+void require_topk(const mbx::BlockShape& s, int64_t topk) {
+    MBX_REQUIRE(topk >= 0 && topk <= 65536, "topk must be in [0, 65536]");
+    const int64_t q_blocks = (s.nq + MBX_ATTENTION_BLOCK_Q - 1) / MBX_ATTENTION_BLOCK_Q;
+    MBX_REQUIRE(s.n * s.heads * q_blocks < (int64_t(1) << 31), "too many query blocks");
+}
+
+void require_workspace(const void* p, size_t have, size_t need) {
+    if (need == 0) return;
+    MBX_REQUIRE(have >= need, "workspace of " + std::to_string(have) + " bytes, " + std::to_string(need) + " needed");
+    require_aligned(p, 256, "workspace");
+}
+
 // IEEE binary16 -> binary32 (exact).
 float half_bits_to_float(uint16_t h) {
     uint32_t sign = uint32_t(h & 0x8000u) << 16;
@@ -717,6 +765,122 @@ int32_t mbx_conv_group_norm_affine(mbx_ctx* ctx, const float* x, int64_t n, int6
             mbx::launch_conv_tc(ctx, x, s, weight, bias, pro_scale, pro_shift, pro_silu != 0, residual, out, act);
             gn_affine_impl(ctx, out, n, ho, wo, c_out, groups, eps, gamma, beta, add, scale_out, shift_out);
         }
+    });
+}
+
+int32_t mbx_qkv_norm_rope(mbx_ctx* ctx, const void* x, int32_t x_dtype, int64_t n, int64_t tokens, int64_t x_stride,
+                          int64_t heads, int64_t kv_heads, int64_t dim, int32_t norm, const float* q_gamma,
+                          const float* k_gamma, float eps, const float* positions, int64_t position_items,
+                          const int64_t axis_dims[3], double theta, int32_t pairing, void* q, void* k, void* v,
+                          int32_t out_dtype) {
+    return guard([&] {
+        require_ctx(ctx);
+        MBX_REQUIRE(n >= 0 && tokens >= 0 && n < kMaxExtent && tokens < kMaxExtent && n * tokens < (int64_t(1) << 34),
+                    "bad shape");
+        MBX_REQUIRE(heads >= 0 && kv_heads >= 0 && heads + kv_heads > 0 && heads <= 65536 && kv_heads <= 65536,
+                    "bad head counts");
+        MBX_REQUIRE(dim > 0 && dim <= mbx::kRopeMaxDim && dim % 8 == 0, "dim must be a multiple of 8, at most 256");
+        require_storage(x_dtype);
+        require_storage(out_dtype);
+        MBX_REQUIRE(x_dtype == MBX_DTYPE_F32 || x_dtype == out_dtype, "f16 and bf16 rows keep their type");
+        MBX_REQUIRE(pairing == MBX_ROPE_ADJACENT || pairing == MBX_ROPE_HALVES, "unknown pairing");
+        require_rows(x, x_stride, (heads + kv_heads + (v ? kv_heads : 0)) * dim, x_dtype, "x");
+        if (norm) MBX_REQUIRE(eps >= 0.0f && std::isfinite(eps), "eps must be finite and not negative");
+        mbx::QkvRope r{x,        x_dtype, out_dtype, n,   tokens,    x_stride,       heads,     kv_heads, dim, norm != 0,
+                       q_gamma,  k_gamma, eps,       positions, position_items, {0, 0, 0}, theta,    pairing, q,
+                       k,        v};
+        if (positions) {
+            require_ptr(axis_dims, "axis_dims");
+            MBX_REQUIRE(position_items == 1 || position_items == n, "position_items must be 1 or n");
+            MBX_REQUIRE(std::isfinite(theta) && theta > 0.0, "theta must be positive");
+            int64_t sum = 0;
+            for (int a = 0; a < 3; ++a) {
+                MBX_REQUIRE(axis_dims[a] >= 0 && axis_dims[a] <= dim && axis_dims[a] % 2 == 0,
+                            "axis_dims must be even and at most dim");
+                r.axis_dims[a] = axis_dims[a];
+                sum += axis_dims[a];
+            }
+            MBX_REQUIRE(sum <= dim, "axis_dims exceed dim");
+        }
+        if (n * tokens == 0) return;
+        require_ptr(x, "x");
+        if (heads > 0) require_aligned(q, 16, "q");
+        if (kv_heads > 0) require_aligned(k, 16, "k");
+        if (kv_heads == 0) r.v = nullptr;
+        if (r.v) require_aligned(r.v, 16, "v");
+        use_device(ctx);
+        mbx::launch_qkv_norm_rope(ctx, r);
+    });
+}
+
+int32_t mbx_block_select_workspace(int64_t n, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t dim,
+                                   int64_t block_k, size_t* bytes) {
+    return guard([&] {
+        require_ptr(bytes, "bytes");
+        *bytes = mbx::block_select_bytes(block_shape(MBX_DTYPE_F32, n, nq, nk, heads, kv_heads, dim, block_k,
+                                                     mbx::kRopeMaxDim));
+    });
+}
+
+int32_t mbx_block_select(mbx_ctx* ctx, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                         int32_t dtype, int64_t n, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
+                         int64_t dim, int64_t block_k, const uint8_t* key_mask, int64_t topk, int32_t* index,
+                         void* workspace, size_t workspace_bytes) {
+    return guard([&] {
+        require_ctx(ctx);
+        const mbx::BlockShape s = block_shape(dtype, n, nq, nk, heads, kv_heads, dim, block_k, mbx::kRopeMaxDim);
+        require_topk(s, topk);
+        require_rows(q, q_stride, heads * dim, dtype, "q");
+        require_rows(k, k_stride, kv_heads * dim, dtype, "k");
+        if (n == 0 || nq == 0 || topk == 0) return;
+        require_ptr(q, "q");
+        if (nk > 0) require_ptr(k, "k");
+        require_ptr(index, "index");
+        require_workspace(workspace, workspace_bytes, mbx::block_select_bytes(s));
+        use_device(ctx);
+        mbx::launch_block_select(ctx, s, q, q_stride, k, k_stride, key_mask, topk, index, workspace);
+    });
+}
+
+int32_t mbx_block_attention_workspace(int32_t dtype, int64_t n, int64_t nq, int64_t nk, int64_t heads,
+                                      int64_t kv_heads, int64_t dim, int64_t block_k, int64_t topk, size_t* bytes) {
+    return guard([&] {
+        require_ptr(bytes, "bytes");
+        const mbx::BlockShape s = block_shape(dtype, n, nq, nk, heads, kv_heads, dim, block_k, 128);
+        require_topk(s, topk);
+        *bytes = mbx::block_attention_bytes(s, topk);
+    });
+}
+
+int32_t mbx_block_attention(mbx_ctx* ctx, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                            const void* v, int64_t v_stride, int32_t dtype, int64_t n, int64_t nq, int64_t nk,
+                            int64_t heads, int64_t kv_heads, int64_t dim, int64_t block_k, const uint8_t* key_mask,
+                            const int32_t* index, int64_t topk, float scale, void* out, void* workspace,
+                            size_t workspace_bytes) {
+    return guard([&] {
+        require_ctx(ctx);
+        const mbx::BlockShape s = block_shape(dtype, n, nq, nk, heads, kv_heads, dim, block_k, 128);
+        require_topk(s, topk);
+        require_rows(q, q_stride, heads * dim, dtype, "q");
+        require_rows(k, k_stride, kv_heads * dim, dtype, "k");
+        require_rows(v, v_stride, kv_heads * dim, dtype, "v");
+        MBX_REQUIRE(std::isfinite(scale), "scale must be finite");
+        if (n == 0 || nq == 0) return;
+        require_ptr(q, "q");
+        require_aligned(out, 16, "out");
+        if (nk == 0 || topk == 0) {  // no key for any row
+            use_device(ctx);
+            check_cuda(cudaMemsetAsync(out, 0, (size_t)(n * nq * heads * dim) * storage_size(dtype), ctx->stream),
+                       "cudaMemsetAsync");
+            return;
+        }
+        require_ptr(k, "k");
+        require_ptr(v, "v");
+        require_ptr(index, "index");
+        require_workspace(workspace, workspace_bytes, mbx::block_attention_bytes(s, topk));
+        use_device(ctx);
+        mbx::launch_block_attention(ctx, s, q, q_stride, k, k_stride, v, v_stride, key_mask, index, topk, scale, out,
+                                    workspace);
     });
 }
 

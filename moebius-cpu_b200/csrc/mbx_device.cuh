@@ -1,6 +1,8 @@
 // Device-side helpers shared by the kernels.
 #pragma once
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -51,6 +53,71 @@ struct ChanStationary {
 
 __device__ __forceinline__ float4 f4_fma(float4 a, float4 b, float4 c) {
     return make_float4(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y), fmaf(a.z, b.z, c.z), fmaf(a.w, b.w, c.w));
+}
+
+// Eight consecutive elements of any of the storage types as f32, and back (rounded to nearest):
+// one or two 16-byte accesses, so p must be 16-byte aligned.
+struct Raw8f {
+    float4 a, b;
+};
+template <class T>
+struct Raw8 {
+    using type = uint4;
+};
+template <>
+struct Raw8<float> {
+    using type = Raw8f;
+};
+
+__device__ __forceinline__ Raw8f load_raw8(const float* p) {
+    return Raw8f{__ldg(reinterpret_cast<const float4*>(p)), __ldg(reinterpret_cast<const float4*>(p) + 1)};
+}
+template <class T>
+__device__ __forceinline__ uint4 load_raw8(const T* p) {
+    return __ldg(reinterpret_cast<const uint4*>(p));
+}
+
+template <class T>
+__device__ __forceinline__ void widen8(const typename Raw8<T>::type& r, float (&v)[8]);
+template <>
+__device__ __forceinline__ void widen8<float>(const Raw8f& r, float (&v)[8]) {
+    v[0] = r.a.x, v[1] = r.a.y, v[2] = r.a.z, v[3] = r.a.w;
+    v[4] = r.b.x, v[5] = r.b.y, v[6] = r.b.z, v[7] = r.b.w;
+}
+template <>
+__device__ __forceinline__ void widen8<__half>(const uint4& r, float (&v)[8]) {
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+template <>
+__device__ __forceinline__ void widen8<__nv_bfloat16>(const uint4& r, float (&v)[8]) {
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+}
+
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    __nv_bfloat162 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
 }
 
 }  // namespace mbx

@@ -158,6 +158,38 @@ void launch_softmax_rows(mbx_ctx* ctx, float* x, int64_t rows, int64_t n, float 
 void launch_split_to_param(mbx_ctx* ctx, const float* b, int64_t n, int64_t k, bool b_is_kn, mbx_param* p);
 void launch_scale_add(mbx_ctx* ctx, const float* x, int64_t len, float mul, float add, float* out);
 
+// Image-token attention (k_qkv_rope.cu, k_block_select.cu, k_block_attention.cu).
+constexpr int kRopeMaxDim = 256;
+struct QkvRope {
+    const void* x;
+    int x_dtype, out_dtype;
+    int64_t n, tokens, x_stride, heads, kv_heads, dim;
+    int norm;
+    const float *q_gamma, *k_gamma;
+    float eps;
+    const float* positions;
+    int64_t position_items;
+    int64_t axis_dims[3];
+    double theta;
+    int pairing;
+    void *q, *k, *v;
+};
+void launch_qkv_norm_rope(mbx_ctx* ctx, const QkvRope& r);
+
+struct BlockShape {
+    int dtype;
+    int64_t n, nq, nk, heads, kv_heads, dim, block_k;
+};
+inline size_t align256(size_t bytes) { return (bytes + 255) & ~size_t(255); }
+// Scratch bytes of the two block operators (the caller's, so that captured graphs need not share any).
+size_t block_select_bytes(const BlockShape& s);
+size_t block_attention_bytes(const BlockShape& s, int64_t topk);
+void launch_block_select(mbx_ctx* ctx, const BlockShape& s, const void* q, int64_t q_stride, const void* k,
+                         int64_t k_stride, const uint8_t* key_mask, int64_t topk, int32_t* index, void* workspace);
+void launch_block_attention(mbx_ctx* ctx, const BlockShape& s, const void* q, int64_t q_stride, const void* k,
+                            int64_t k_stride, const void* v, int64_t v_stride, const uint8_t* key_mask,
+                            const int32_t* index, int64_t topk, float scale, void* out, void* workspace);
+
 // λ layers (k_lambda.cu). lambda_content needs scratch: pmax and psum
 // [items][chunks][k], plam [items][chunks][k][vd] with chunks = lambda_chunks(rows).
 int64_t lambda_chunks(int64_t rows);
