@@ -11,6 +11,7 @@
 // (output, maximum, sum) a second kernel joins.
 #include <algorithm>
 
+#include "block_attention.h"
 #include "mbx_device.cuh"
 #include "mbx_internal.h"
 
@@ -18,18 +19,6 @@ namespace mbx {
 namespace {
 
 constexpr int kRowWarps = 4;
-
-struct AttnArgs {
-    const void *q, *k, *v;
-    int64_t q_stride, k_stride, v_stride, nq, nk, topk;
-    int heads, kv_heads, dim, block_k, k_blocks, q_blocks;
-    const uint8_t* mask;   // [n][nk] or null
-    const int32_t* index;  // [n][heads][q_blocks][topk]
-    float scale;           // scale · log2(e): exponentials are 2^x
-    void* out;             // [n][nq][heads][dim]
-    float* part;           // splits > 1: [n][nq][heads][splits][dim + 2], then the joined result goes to out
-    int splits;
-};
 
 // Lanes of a key's group: the power of two that holds dim / 8.
 template <class T, int R>
@@ -155,12 +144,27 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, i
 }
 
 constexpr int kRowsR = 4;
+constexpr int64_t kSms = 148;
 
-// Splits of the listed blocks: enough CTAs to fill the card twice over (148 SMs), never more than the listed blocks.
-int row_splits(const BlockShape& s, int64_t topk) {
-    const int64_t ctas = s.n * s.heads * ((s.nq + kRowsR - 1) / kRowsR);
-    const int64_t want = (2 * 148 + ctas - 1) / std::max<int64_t>(ctas, 1);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, topk), 64));
+// Which kernel takes a problem, and over how many CTAs a list is split: enough to fill the card
+// twice over, never more than there are blocks (rows) or tiles of 128 keys (tensor cores).
+struct Plan {
+    bool rows;
+    int splits;
+    size_t part_bytes, split_bytes;
+};
+
+Plan plan_of(const BlockShape& s, int64_t topk) {
+    Plan p{};
+    p.rows = s.dtype == MBX_DTYPE_F32 && s.nq < 16;
+    const int64_t tile = p.rows ? kRowsR : MBX_ATTENTION_BLOCK_Q;
+    const int64_t ctas = std::max<int64_t>(1, s.n * s.heads * ((s.nq + tile - 1) / tile));
+    const int64_t pieces = p.rows ? topk : (topk * s.block_k + 127) / 128;
+    p.splits = (int)std::max<int64_t>(1, std::min({(2 * kSms + ctas - 1) / ctas, pieces, int64_t(64)}));
+    if (p.splits > 1)
+        p.part_bytes = align256(sizeof(float) * (size_t)(s.n * s.nq * s.heads) * p.splits * (s.dim + 2));
+    if (!p.rows && s.dtype == MBX_DTYPE_F32) p.split_bytes = attention_split_bytes(s);
+    return p;
 }
 
 template <class T>
@@ -174,23 +178,26 @@ void launch_rows(mbx_ctx* ctx, const AttnArgs& a, int64_t n) {
     ensure_smem_limit((const void*)attention_rows_kernel<T, kRowsR>, (int)smem, "attention_rows");
     attention_rows_kernel<T, kRowsR><<<(unsigned)ctas, kRowWarps * 32, smem, ctx->stream>>>(a, group);
     after_launch(ctx, "attention_rows");
-    if (a.splits > 1) {
-        const int64_t rows = n * a.nq * a.heads;
-        attention_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, ctx->stream>>>(a, rows);
-        after_launch(ctx, "attention_join");
-    }
+}
+
+template <class T>
+void launch_join(mbx_ctx* ctx, const AttnArgs& a, int64_t n) {
+    const int64_t rows = n * a.nq * a.heads;
+    attention_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, ctx->stream>>>(a, rows);
+    after_launch(ctx, "attention_join");
 }
 
 }  // namespace
 
 size_t block_attention_bytes(const BlockShape& s, int64_t topk) {
-    const int splits = row_splits(s, topk);
-    return splits > 1 ? align256(sizeof(float) * (size_t)(s.n * s.nq * s.heads) * splits * (s.dim + 2)) : 0;
+    const Plan p = plan_of(s, topk);
+    return p.part_bytes + p.split_bytes;
 }
 
 void launch_block_attention(mbx_ctx* ctx, const BlockShape& s, const void* q, int64_t q_stride, const void* k,
                             int64_t k_stride, const void* v, int64_t v_stride, const uint8_t* key_mask,
                             const int32_t* index, int64_t topk, float scale, void* out, void* workspace) {
+    const Plan p = plan_of(s, topk);
     AttnArgs a{};
     a.q = q, a.k = k, a.v = v;
     a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
@@ -202,10 +209,15 @@ void launch_block_attention(mbx_ctx* ctx, const BlockShape& s, const void* q, in
     a.scale = scale * 1.4426950408889634f;  // log2(e)
     a.out = out;
     a.part = static_cast<float*>(workspace);
-    a.splits = row_splits(s, topk);
-    if (s.dtype == MBX_DTYPE_F32) return launch_rows<float>(ctx, a, s.n);
-    if (s.dtype == MBX_DTYPE_F16) return launch_rows<__half>(ctx, a, s.n);
-    launch_rows<__nv_bfloat16>(ctx, a, s.n);
+    a.splits = p.splits;
+    if (p.rows)
+        launch_rows<float>(ctx, a, s.n);
+    else
+        launch_attention_tc(ctx, a, s.dtype, s.n, static_cast<uint8_t*>(workspace) + p.part_bytes);
+    if (p.splits == 1) return;
+    if (s.dtype == MBX_DTYPE_F32) return launch_join<float>(ctx, a, s.n);
+    if (s.dtype == MBX_DTYPE_F16) return launch_join<__half>(ctx, a, s.n);
+    launch_join<__nv_bfloat16>(ctx, a, s.n);
 }
 
 }  // namespace mbx

@@ -1,0 +1,700 @@
+// Block attention on the sm_100a tensor cores (tcgen05.mma, accumulators and weights in TMEM,
+// TMA-fed operands).
+//
+// A CTA takes one query block (128 rows) of one (item, head), or a share of its list, and walks
+// the listed key blocks in tiles of 128 keys (128 / block_k blocks a tile, each its own TMA box,
+// so any block size feeds the same tile). Six warps:
+//   warps 0-3  softmax: a thread owns a query row (a TMEM lane). It reads S from TMEM, keeps the
+//              running maximum and sum in f32 registers and writes the weights 2^(c·s − c·m)
+//              back over S, as the second product's left operand.
+//   warp 4     producer: TMA for Q once and for K, V of every tile; the tile's bits of valid keys.
+//   warp 5     MMA issuer (one thread) and TMEM allocation.
+// TMEM (256 columns): S, then P, in columns 0-127, O behind. Shared memory: Q, K and V in
+// 128-byte-swizzled panels of 64 channels; V serves as the N-major operand as it lies, so nothing
+// is transposed. Two CTAs share an SM (one for f32 with more than 64 channels): while one computes
+// weights, the other's products run.
+//
+// 16-bit operands: P is rounded to their type (half a step of a weight, beside half a step of the
+// result at the end). The weights are relative to a reference that is raised only when a row's
+// maximum outgrows it by 2^8, so O, which accumulates in TMEM over the whole list, is rarely
+// rescaled.
+//
+// f32 operands: q, k and v are split beforehand into two f16 parts, after a power-of-two scale that
+// brings the largest magnitude of the head to 2^14: a value is held to 2^-22 of itself, or to
+// 2^-39 of the largest. Three products (lo·hi, hi·lo, hi·hi; lo·lo is 2^-22 of the whole), and the
+// weights in two parts after a scale of 2^13. The tensor core truncates as it adds into its f32
+// accumulator, so a long sum there drifts by about 2^-25 a step: each tile's P·V starts a fresh
+// accumulator and the softmax threads add it to f32 registers, rounding to nearest.
+//
+// Masked keys: S becomes −inf; their V rows become zero in shared memory (16-bit) or while
+// splitting (f32), since zero times what a mask hides may be NaN.
+// Every wait is bounded; on timeout the CTA records the error, waits (bounded) for its copies and
+// MMAs in flight, frees TMEM and returns.
+#include <algorithm>
+#include <type_traits>
+
+#include "block_attention.h"
+#include "mbx_device.cuh"
+#include "mbx_tc.cuh"
+
+namespace mbx {
+namespace {
+
+constexpr int kRows = MBX_ATTENTION_BLOCK_Q;
+constexpr int kKeys = 128;              // keys of a tile
+constexpr uint32_t kPanel = 128 * 128;  // bytes of 128 rows × 64 channels
+constexpr int kThreads = 192;
+constexpr uint32_t kTmemCols = 256;
+constexpr uint32_t kColO = 128;
+constexpr int kMaskSlots = 4;
+constexpr float kLazy = 8.0f;    // log2 of the largest 16-bit weight
+constexpr int kScaleExp = 14;    // f32 operands: the largest magnitude becomes 2^14 .. 2^15
+constexpr int kWeightExp = 13;   // f32 operands: weights are scaled by 2^13
+
+struct TcArgs {
+    AttnArgs a;
+    const uint32_t* amax;  // f32 operands: bits of the largest magnitudes, q [n][heads], k and v [n][kv_heads]
+    int64_t n;
+    int* err;
+};
+
+template <int PANELS, bool SPLIT>
+constexpr int stages_of() {
+    return !SPLIT && PANELS == 1 ? 2 : 1;
+}
+
+template <int PANELS, bool SPLIT>
+constexpr int smem_of() {
+    return (int)(PANELS * (SPLIT ? 2 : 1) * kPanel) * (1 + 2 * stages_of<PANELS, SPLIT>()) + 1024;
+}
+
+// Columns of the warp's 32 lanes, complete on return: the wait is part of the statement, so that nothing that uses the
+// registers can be moved before it.
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15 "
+        "}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_wait(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31 "
+        "}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld128_wait(uint32_t taddr, uint32_t (&r)[128]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, "
+        "%40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, "
+        "%59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, "
+        "%78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, "
+        "%97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, "
+        "%113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127 "
+        "}, [%128];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]),
+          "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]),
+          "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]),
+          "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]),
+          "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16_u32(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {"
+        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16 "
+        "};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The exponent of the power of two that scales a head whose largest magnitude has these bits.
+__device__ __forceinline__ int scale_exponent(uint32_t bits) {
+    if (bits == 0) return 0;
+    return min(kScaleExp + 127 - max((int)(bits >> 23), 1), 126);
+}
+
+// Shared-memory descriptor of an N-major operand (rows are K): 64-channel panels of 128-byte rows,
+// 128-byte swizzle; 8-row groups 1024 bytes apart (SBO), panels kPanel apart (LBO).
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3ffffu) >> 4);
+    d |= (uint64_t)(kPanel >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// Instruction descriptor, kind::f16: D f32, A and B both f16 or both bf16, M = 128, N = n.
+__device__ __forceinline__ uint32_t idesc_16(bool bf16, int n, bool negate_a, bool b_mn) {
+    return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)negate_a << 13) |
+           ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_16_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_16_ts(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(bd), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <class OUT>
+constexpr bool is_f32() {
+    return std::is_same<OUT, float>::value;
+}
+
+// OUT: the type of the tensors; the operands' type is OUT, or f16 parts where OUT is float.
+template <class OUT, int PANELS>
+__global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2)
+    attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcArgs args) {
+    constexpr bool SPLIT = is_f32<OUT>();
+    constexpr bool BF16 = std::is_same<OUT, __nv_bfloat16>::value;
+    constexpr int PLANES = SPLIT ? 2 : 1;
+    constexpr int STAGES = stages_of<PANELS, SPLIT>();
+    constexpr uint32_t OP = PANELS * PLANES * kPanel;  // bytes of one operand's tile
+    constexpr int DCOLS = PANELS * 64;
+    using Part = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    const AttnArgs& a = args.a;
+
+    enum {
+        kKFull = 0,
+        kKEmpty = kKFull + STAGES,
+        kVFull = kKEmpty + STAGES,
+        kVEmpty = kVFull + STAGES,
+        kVClean = kVEmpty + STAGES,
+        kMFull = kVClean + STAGES,
+        kMEmpty = kMFull + kMaskSlots,
+        kQFull = kMEmpty + kMaskSlots,
+        kSFull,
+        kPFull,
+        kOFull,
+        kFin,
+        kBars
+    };
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[kBars];
+    __shared__ uint32_t valid[kMaskSlots][4];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag, listed;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t sv = base, sk = sv + STAGES * OP, sq = sk + STAGES * OP;
+    const uint32_t bar0 = smem_u32(bars);
+    auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t cta = blockIdx.x / a.splits;  // (item, head, query block)
+    const int split = (int)(blockIdx.x - cta * a.splits);
+    const int qb = (int)(cta % a.q_blocks);
+    const int h = (int)(cta / a.q_blocks % a.heads);
+    const int item = (int)(cta / a.q_blocks / a.heads);
+    const int kh = h / (a.heads / a.kv_heads);
+    const int32_t* list = a.index + cta * a.topk;
+    const uint8_t* mask = a.mask ? a.mask + (int64_t)item * a.nk : nullptr;
+    const bool cleans = !SPLIT && mask != nullptr;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(bar(kKFull + i), 1), mbar_init(bar(kKEmpty + i), 1);
+            mbar_init(bar(kVFull + i), 1), mbar_init(bar(kVEmpty + i), 1), mbar_init(bar(kVClean + i), 1);
+        }
+        for (int i = 0; i < kMaskSlots; ++i) mbar_init(bar(kMFull + i), 1), mbar_init(bar(kMEmpty + i), 4);
+        mbar_init(bar(kQFull), 1), mbar_init(bar(kSFull), 1), mbar_init(bar(kPFull), 128);
+        mbar_init(bar(kOFull), 1), mbar_init(bar(kFin), 1);
+        abort_flag = 0, listed = 0;
+        fence_mbarrier_init();
+    }
+    if (warp == 5) {
+        tmem_alloc(smem_u32(&tmem_slot), kTmemCols);
+        tmem_relinquish();
+    }
+    __syncthreads();
+    {  // entries up to the last one that names a block
+        int last = 0;
+        for (int e = threadIdx.x; e < (int)a.topk; e += kThreads)
+            if ((uint32_t)list[e] < (uint32_t)a.k_blocks) last = e + 1;
+        last = __reduce_max_sync(0xffffffffu, last);
+        if (lane == 0 && last > 0) atomicMax(&listed, last);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int per_tile = kKeys / a.block_k;
+    const int all_tiles = (listed + per_tile - 1) / per_tile;
+    const int t0 = (int)((int64_t)all_tiles * split / a.splits);
+    const int tiles = (int)((int64_t)all_tiles * (split + 1) / a.splits) - t0;
+    volatile int* abort_p = &abort_flag;
+    auto wait = [&](int b, int phase, int site) {
+        return mbar_wait(bar(b), (uint32_t)phase & 1u, args.err, site, abort_p, true, kWaitLimit, kKAttention);
+    };
+
+    // The same answer in every lane: what follows is done by whole warps.
+    auto warp_wait = [&](int b, int phase, int site) { return __all_sync(0xffffffffu, wait(b, phase, site)) != 0; };
+
+    if (warp < 4) {
+        // ---------------------------------------------------------------- softmax
+        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        // A negative scale negates Q in the instruction descriptor. The least normal value in place of 0 (a scale of
+        // 0, or far below what matters) keeps −inf · c = −inf.
+        float c = fabsf(a.scale);
+        int ev = 0;
+        if (SPLIT) {
+            const uint32_t* kv = args.amax + args.n * a.heads + (int64_t)item * a.kv_heads + kh;
+            ev = scale_exponent(kv[args.n * a.kv_heads]);
+            c = ldexpf(c, -(scale_exponent(args.amax[(int64_t)item * a.heads + h]) + scale_exponent(*kv)));
+        }
+        c = fmaxf(c, 1.17549435e-38f);
+        float ref = -INFINITY, l = 0.0f;  // what the weights are relative to, in units of S; their sum
+        float acc[SPLIT ? DCOLS : 1];
+#pragma unroll
+        for (int i = 0; i < (SPLIT ? DCOLS : 1); ++i) acc[i] = 0.0f;
+        auto fold = [&] {  // f32: the last tile's product joins the row's sum
+#pragma unroll
+            for (int i = 0; i < (SPLIT ? DCOLS : 0); i += 32) {
+                uint32_t o[32];
+                tmem_ld32_wait(lanes + kColO + i, o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) acc[SPLIT ? i + e : 0] += __uint_as_float(o[e]);
+            }
+        };
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            const int slot = j % kMaskSlots;
+            ok = warp_wait(kMFull + slot, j / kMaskSlots, 20);
+            if (!ok) break;
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = *(volatile uint32_t*)&valid[slot][i];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kMEmpty + slot));
+            const bool full = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu;
+            ok = warp_wait(kSFull, j, 21);  // this tile's S; the last tile's P·V was complete before it was begun
+            if (!ok) break;
+            tc_fence_after();
+            if (SPLIT && j > 0) fold();
+            constexpr int CH = SPLIT ? 32 : 128;  // columns in registers at a time
+            uint32_t s[CH];
+            float top = -INFINITY;
+            auto load = [&](int q) {
+                if constexpr (SPLIT)
+                    tmem_ld32_wait(lanes + q * CH, s);
+                else
+                    tmem_ld128_wait(lanes, s);
+                if (!full) {
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) {
+                        const uint32_t word = CH == 128 ? w[i >> 5] : (q == 0 ? w[0] : q == 1 ? w[1] : q == 2 ? w[2] : w[3]);
+                        if (!(word >> (i & 31) & 1u)) s[i] = 0xff800000u;
+                    }
+                }
+            };
+#pragma unroll
+            for (int q = 0; q < 128 / CH; ++q) {
+                load(q);
+                float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < CH; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(s[i]));
+                top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+            }
+            // Raise the reference: to every new maximum (f32), or when a weight would pass 2^8.
+            const bool raise = SPLIT || ref == -INFINITY ? top > ref : (top - ref) * c > kLazy;
+            if (__any_sync(0xffffffffu, raise)) {
+                const float f = !raise ? 1.0f : (ref == -INFINITY ? 0.0f : ex2((ref - top) * c));
+                if (raise) ref = top;
+                l *= f;
+                if (SPLIT) {
+#pragma unroll
+                    for (int i = 0; i < (SPLIT ? DCOLS : 0); ++i) acc[SPLIT ? i : 0] *= f;
+                } else if (j > 0) {
+#pragma unroll
+                    for (int i = 0; i < DCOLS; i += 16) {
+                        uint32_t o[16];
+                        tmem_ld16_wait(lanes + kColO + i, o);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st16_u32(lanes + kColO + i, o);
+                    }
+                }
+            }
+            const float mc = (ref == -INFINITY ? 0.0f : ref) * c - (SPLIT ? (float)kWeightExp : 0.0f);
+            float sum[4] = {};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {  // 32 keys: 16 columns of P, and at f32 16 more of its low part
+                if (SPLIT) load(q);
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int at = (SPLIT ? 0 : q * 32) + 2 * i;
+                    const float p0 = ex2(fmaf(__uint_as_float(s[at]), c, -mc));
+                    const float p1 = ex2(fmaf(__uint_as_float(s[at + 1]), c, -mc));
+                    sum[i & 1] += p0, sum[2 + (i & 1)] += p1;
+                    hi[i] = pack2(p0, p1, Part());
+                    if (SPLIT) {
+                        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+                        lo[i] = pack2(p0 - b.x, p1 - b.y, Part());
+                    }
+                }
+                // f32 parts lie over their own 32 columns of S, whose other columns are still to be read.
+                tmem_st16_u32(lanes + q * (SPLIT ? 32 : 16), hi);
+                if (SPLIT) tmem_st16_u32(lanes + q * 32 + 16, lo);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar(kPFull));
+        }
+        if (ok && tiles > 0) ok = warp_wait(kOFull, tiles - 1, 22);
+        if (ok) {
+            tc_fence_after();
+            const int64_t row = (int64_t)qb * kRows + warp * 32 + lane;
+            const bool store = row < a.nq;
+            const int64_t at = ((int64_t)item * a.nq + row) * a.heads + h;
+            if (SPLIT && tiles > 0) fold();
+            // One factor for the row: 1 / l, or for a share of the list the weights' own scale taken out.
+            const float f = a.splits > 1 ? (SPLIT ? ldexpf(1.0f, -ev - kWeightExp) : 1.0f)
+                                         : (l == 0.0f ? 0.0f : (SPLIT ? ldexpf(1.0f, -ev) : 1.0f) / l);
+            float* part = a.part + (at * a.splits + split) * (a.dim + 2);
+            if (a.splits > 1 && store) {
+                part[a.dim] = ref == -INFINITY ? ref : ref * c;
+                part[a.dim + 1] = SPLIT ? ldexpf(l, -kWeightExp) : l;
+            }
+#pragma unroll
+            for (int i = 0; i < DCOLS; i += 32) {
+                uint32_t o[32];
+                if (!SPLIT && tiles > 0) tmem_ld32_wait(lanes + kColO + i, o);
+#pragma unroll
+                for (int g = 0; g < 32; g += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float v = SPLIT ? acc[SPLIT ? i + g + e : 0] : __uint_as_float(o[g + e]);
+                        y[e] = l == 0.0f ? 0.0f : v * f;
+                    }
+                    if (!store || i + g >= a.dim) continue;
+                    if (a.splits > 1) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) part[i + g + e] = y[e];
+                    } else {
+                        store8(static_cast<OUT*>(a.out) + at * a.dim + i + g, y);
+                    }
+                }
+            }
+        }
+    } else if (warp == 4) {
+        // ---------------------------------------------------------------- producer
+        auto load_tile = [&](const CUtensorMap* map, uint32_t dst, int full_bar, int head, int token, int boxes,
+                             int rows) {  // `boxes` lanes bring `rows` rows each
+            if (lane == 0) mbar_arrive_expect_tx(bar(full_bar), OP);
+            __syncwarp();
+            if (lane < boxes) {
+#pragma unroll
+                for (int p = 0; p < PLANES * PANELS; ++p)
+                    tma_load_4d(dst + p * kPanel + lane * rows * 128, map, (p % PANELS) * 64, head, token,
+                                item + (p / PANELS) * (int)args.n, bar(full_bar));
+            }
+            __syncwarp();
+        };
+        int q_done = 0, k_done = 0, v_done = 0;
+        if (tiles > 0) {
+            load_tile(&map_q, sq, kQFull, h, qb * kRows, 1, kRows);
+            q_done = 1;
+        }
+        for (int j = 0; j < tiles; ++j) {
+            const int st = j % STAGES, ph = j / STAGES, slot = j % kMaskSlots;
+            int token = (int)a.nk;  // past the last key: zeros
+            if (lane < per_tile) {
+                const int e = (t0 + j) * per_tile + lane;
+                const int blk = e < listed ? list[e] : -1;
+                if ((uint32_t)blk < (uint32_t)a.k_blocks) token = blk * a.block_k;
+            }
+            if (j >= STAGES && !warp_wait(kKEmpty + st, ph - 1, 23)) break;
+            load_tile(&map_k, sk + st * OP, kKFull + st, kh, token, per_tile, a.block_k);
+            k_done = j + 1;
+            if (j >= kMaskSlots && !warp_wait(kMEmpty + slot, j / kMaskSlots - 1, 24)) break;
+            uint32_t w[4];
+            bool hidden = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = i * 32 + lane;
+                const int64_t t = (int64_t)__shfl_sync(0xffffffffu, token, key / a.block_k) + key % a.block_k;
+                const bool in = t < a.nk, keep = in && (!mask || mask[t]);
+                w[i] = __ballot_sync(0xffffffffu, keep);
+                hidden |= in && !keep;
+            }
+            hidden = __any_sync(0xffffffffu, hidden);
+            if (lane == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *(volatile uint32_t*)&valid[slot][i] = w[i];
+                mbar_arrive(bar(kMFull + slot));
+            }
+            if (j >= STAGES && !warp_wait(kVEmpty + st, ph - 1, 25)) break;
+            load_tile(&map_v, sv + st * OP, kVFull + st, kh, token, per_tile, a.block_k);
+            v_done = j + 1;
+            if (cleans) {
+                if (hidden) {
+                    if (!warp_wait(kVFull + st, ph, 26)) break;
+                    for (int r = 0; r < kKeys; ++r) {
+                        if (w[r >> 5] >> (r & 31) & 1u) continue;
+#pragma unroll
+                        for (int p = 0; p < PANELS; ++p)
+                            *reinterpret_cast<uint32_t*>(gbase + st * OP + p * kPanel + r * 128 + lane * 4) = 0;
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive(bar(kVClean + st));
+            }
+        }
+        __syncwarp();
+        if (*abort_p && lane == 0) {  // copies in flight land before the CTA's memory is given up
+            const long long deadline = clock64() + kWaitLimit;
+            if (q_done) drain_wait(bar(kQFull), 0, deadline, args.err, 27, kKAttention);
+            for (int i = std::max(0, k_done - STAGES); i < k_done; ++i)
+                drain_wait(bar(kKFull + i % STAGES), (uint32_t)(i / STAGES) & 1u, deadline, args.err, 27, kKAttention);
+            for (int i = std::max(0, v_done - STAGES); i < v_done; ++i)
+                drain_wait(bar(kVFull + i % STAGES), (uint32_t)(i / STAGES) & 1u, deadline, args.err, 27, kKAttention);
+        }
+    } else if (lane == 0 && tiles > 0) {
+        // ---------------------------------------------------------------- MMA issuer
+        const int k_steps = (a.dim + 15) / 16;
+        const uint32_t idesc_s = idesc_16(BF16, kKeys, a.scale < 0.0f, false);
+        const uint32_t idesc_o = idesc_16(BF16, k_steps * 16, false, true);
+        bool ok = wait(kQFull, 0, 28);
+        for (int j = 0; ok && j < tiles; ++j) {
+            const int st = j % STAGES, ph = j / STAGES;
+            ok = wait(kKFull + st, ph, 29);
+            // S lies over the P that the last tile's product reads.
+            if (ok && j > 0) ok = wait(kOFull, j - 1, 30);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int p = SPLIT ? 0 : 2; p < 3; ++p) {  // lo·hi, hi·lo, hi·hi
+                const uint32_t qa = sq + (p == 0 ? PANELS * kPanel : 0);
+                const uint32_t ka = sk + st * OP + (p == 1 ? PANELS * kPanel : 0);
+                for (int s = 0; s < k_steps; ++s) {
+                    const uint32_t off = (uint32_t)(s >> 2) * kPanel + (uint32_t)(s & 3) * 32u;
+                    mma_16_ss(tmem, sw128_desc(qa + off), sw128_desc(ka + off), idesc_s,
+                              (p > (SPLIT ? 0 : 2) || s > 0) ? 1u : 0u);
+                }
+            }
+            mma_commit(bar(kKEmpty + st));
+            mma_commit(bar(kSFull));
+            ok = wait(kVFull + st, ph, 31);
+            if (ok && cleans) ok = wait(kVClean + st, ph, 32);
+            if (ok) ok = wait(kPFull, j, 33);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int p = SPLIT ? 0 : 2; p < 3; ++p) {
+                const uint32_t va = sv + st * OP + (p == 1 ? PANELS * kPanel : 0);
+#pragma unroll
+                for (int s = 0; s < kKeys / 16; ++s) {
+                    const uint32_t pa = SPLIT ? (uint32_t)(s >> 1) * 32u + (uint32_t)(s & 1) * 8u + (p == 0 ? 16u : 0u)
+                                              : (uint32_t)s * 8u;
+                    const bool fresh = s == 0 && (SPLIT ? p == 0 : j == 0);
+                    mma_16_ts(tmem + kColO, tmem + pa, sw128_desc_mn(va + (uint32_t)s * 2048u), idesc_o,
+                              fresh ? 0u : 1u);
+                }
+            }
+            mma_commit(bar(kVEmpty + st));
+            mma_commit(bar(kOFull));
+        }
+        if (!ok) {  // MMAs in flight finish before TMEM is freed
+            mma_commit(bar(kFin));
+            drain_wait(bar(kFin), 0, clock64() + kWaitLimit, args.err, 34, kKAttention);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 5) tmem_dealloc(tmem, kTmemCols);
+}
+
+// ------------------------------------------------------------------------------------ f32 operands
+
+struct SplitArgs {
+    const float *x[3];           // q, k, v
+    int64_t stride[3], rows[3];  // elements between rows; rows of an item
+    int heads[3];
+    __half* parts[3];            // [2][n][rows][heads][dim]
+    uint32_t* amax;
+    int64_t n;
+    int dim;
+    const uint8_t* mask;         // k and v: rows that count
+};
+
+constexpr int kSplitRows = 64;
+
+// The largest finite magnitude of every (item, head) of q, k and v; the block's y is 3 · (group of 32 chunks) + tensor.
+__global__ void __launch_bounds__(256) attention_amax_kernel(const __grid_constant__ SplitArgs a) {
+    const int t = blockIdx.y % 3, chunk = blockIdx.y / 3 * 32 + (threadIdx.x & 31);
+    const int64_t item = blockIdx.z, r0 = (int64_t)blockIdx.x * kSplitRows;
+    if (r0 >= a.rows[t] || chunk * 8 >= a.heads[t] * a.dim) return;
+    const int64_t r1 = min(r0 + kSplitRows, a.rows[t]);
+    uint32_t top = 0;
+#pragma unroll 4
+    for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
+        if (t > 0 && a.mask && !a.mask[item * a.rows[t] + r]) continue;
+        float v[8];
+        widen8<float>(load_raw8(a.x[t] + (item * a.rows[t] + r) * a.stride[t] + chunk * 8), v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+            if (b < 0x7f800000u) top = max(top, b);
+        }
+    }
+    const int64_t first = t == 0 ? 0 : a.n * (a.heads[0] + (t - 1) * a.heads[1]);
+    if (top) atomicMax(a.amax + first + item * a.heads[t] + chunk * 8 / a.dim, top);
+}
+
+// x · 2^e as two f16 parts; rows that the mask hides become zero.
+__global__ void __launch_bounds__(256) attention_split_kernel(const __grid_constant__ SplitArgs a) {
+    const int t = blockIdx.y % 3, chunk = blockIdx.y / 3 * 32 + (threadIdx.x & 31);
+    const int64_t item = blockIdx.z, r0 = (int64_t)blockIdx.x * kSplitRows;
+    const int width = a.heads[t] * a.dim;
+    if (r0 >= a.rows[t] || chunk * 8 >= width) return;
+    const int64_t first = t == 0 ? 0 : a.n * (a.heads[0] + (t - 1) * a.heads[1]);
+    const int e = scale_exponent(a.amax[first + item * a.heads[t] + chunk * 8 / a.dim]);
+    const float f = ldexpf(1.0f, e);
+    const int64_t r1 = min(r0 + kSplitRows, a.rows[t]), plane = a.n * a.rows[t] * width;
+#pragma unroll 4
+    for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
+        const int64_t row = item * a.rows[t] + r;
+        float v[8], lo[8];
+        if (t > 0 && a.mask && !a.mask[row]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        } else {
+            widen8<float>(load_raw8(a.x[t] + row * a.stride[t] + chunk * 8), v);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] *= f;
+            lo[i] = v[i] - __half2float(__float2half_rn(v[i]));
+        }
+        __half* out = a.parts[t] + row * width + chunk * 8;
+        store8(out, v);
+        store8(out + plane, lo);
+    }
+}
+
+// A map over [items][rows][heads][dim] 16-bit values, boxes of 64 channels × one head × box_rows rows.
+void encode_heads(CUtensorMap* map, const void* base, bool bf16, int64_t items, int64_t rows, int64_t heads,
+                  int64_t dim, int64_t stride, int box_rows) {
+    const uint64_t dims[4] = {(uint64_t)dim, (uint64_t)heads, (uint64_t)rows, (uint64_t)items};
+    const uint64_t strides[3] = {(uint64_t)dim * 2, (uint64_t)stride * 2, (uint64_t)(rows * stride) * 2};
+    const uint32_t box[4] = {64, 1, (uint32_t)box_rows, 1};
+    encode_tensor_map_16(map, base, bf16, 4, dims, strides, box);
+}
+
+template <class OUT, int PANELS>
+void launch_typed(mbx_ctx* ctx, const TcArgs& t, const CUtensorMap (&maps)[3]) {
+    const int64_t ctas = t.n * t.a.heads * t.a.q_blocks * t.a.splits;
+    MBX_REQUIRE(ctas < (int64_t(1) << 31), "block_attention: too many query blocks");
+    constexpr int smem = smem_of<PANELS, is_f32<OUT>()>();
+    ensure_smem_limit((const void*)attention_tc_kernel<OUT, PANELS>, smem, "attention_tc");
+    attention_tc_kernel<OUT, PANELS><<<(unsigned)ctas, kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], t);
+    after_launch(ctx, "attention_tc");
+}
+
+}  // namespace
+
+size_t attention_split_bytes(const BlockShape& s) {
+    return align256(4 * (size_t)(s.n * (s.heads + 2 * s.kv_heads))) + 2 * 2 * (size_t)(s.n * s.nq * s.heads * s.dim) +
+           2 * 2 * 2 * (size_t)(s.n * s.nk * s.kv_heads * s.dim) + 256;
+}
+
+void launch_attention_tc(mbx_ctx* ctx, const AttnArgs& a, int dtype, int64_t n, void* split) {
+    TcArgs t{a, nullptr, n, ctx->dev_err};
+    const void* x[3] = {a.q, a.k, a.v};
+    int64_t stride[3] = {a.q_stride, a.k_stride, a.v_stride};
+    const int64_t rows[3] = {a.nq, a.nk, a.nk}, heads[3] = {a.heads, a.kv_heads, a.kv_heads};
+    int planes = 1;
+    if (dtype == MBX_DTYPE_F32) {
+        planes = 2;
+        SplitArgs s{};
+        s.amax = static_cast<uint32_t*>(split);
+        const size_t amax_bytes = 4 * (size_t)(n * (a.heads + 2 * a.kv_heads));
+        uint8_t* at = static_cast<uint8_t*>(split) + align256(amax_bytes);
+        for (int i = 0; i < 3; ++i) {
+            s.x[i] = static_cast<const float*>(x[i]), s.stride[i] = stride[i], s.rows[i] = rows[i];
+            s.heads[i] = (int)heads[i];
+            s.parts[i] = reinterpret_cast<__half*>(at);
+            at += 2 * 2 * (size_t)(n * rows[i] * heads[i] * a.dim);
+            x[i] = s.parts[i], stride[i] = heads[i] * a.dim;
+        }
+        s.n = n, s.dim = a.dim, s.mask = a.mask;
+        check_cuda(cudaMemsetAsync(s.amax, 0, amax_bytes, ctx->stream), "cudaMemsetAsync");
+        const dim3 grid((unsigned)((std::max(a.nq, a.nk) + kSplitRows - 1) / kSplitRows),
+                        (unsigned)(3 * ((a.heads * a.dim / 8 + 31) / 32)), (unsigned)n);
+        attention_amax_kernel<<<grid, 256, 0, ctx->stream>>>(s);
+        after_launch(ctx, "attention_amax");
+        attention_split_kernel<<<grid, 256, 0, ctx->stream>>>(s);
+        after_launch(ctx, "attention_split");
+        t.amax = s.amax;
+    }
+    CUtensorMap maps[3];
+    for (int i = 0; i < 3; ++i)
+        encode_heads(&maps[i], x[i], dtype == MBX_DTYPE_BF16, planes * n, rows[i], heads[i], a.dim, stride[i],
+                     i == 0 ? kRows : a.block_k);
+    if (dtype == MBX_DTYPE_F32) return a.dim > 64 ? launch_typed<float, 2>(ctx, t, maps) : launch_typed<float, 1>(ctx, t, maps);
+    if (dtype == MBX_DTYPE_F16) return a.dim > 64 ? launch_typed<__half, 2>(ctx, t, maps) : launch_typed<__half, 1>(ctx, t, maps);
+    a.dim > 64 ? launch_typed<__nv_bfloat16, 2>(ctx, t, maps) : launch_typed<__nv_bfloat16, 1>(ctx, t, maps);
+}
+
+}  // namespace mbx

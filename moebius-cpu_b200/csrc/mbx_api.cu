@@ -69,7 +69,7 @@ mbx::BlockShape block_shape(int32_t dtype, int64_t n, int64_t nq, int64_t nk, in
                             int64_t dim, int64_t block_k, int64_t max_dim) {
     require_storage(dtype);
     MBX_REQUIRE(n >= 0 && nq >= 0 && nk >= 0 && nq < kMaxExtent && nk < kMaxExtent, "bad shape");
-    MBX_REQUIRE(heads > 0 && kv_heads > 0 && heads <= 65535 && heads % kv_heads == 0,
+    MBX_REQUIRE(heads > 0 && kv_heads > 0 && heads <= 16384 && heads % kv_heads == 0,
                 "heads must be a multiple of kv_heads");
     MBX_REQUIRE(n <= 65535 && n * heads <= 65535, "n * heads must be at most 65535");
     MBX_REQUIRE(dim > 0 && dim <= max_dim && dim % 8 == 0,

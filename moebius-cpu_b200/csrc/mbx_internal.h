@@ -39,7 +39,7 @@ inline void check_cuda(cudaError_t e, const char* what) {
 // Device-side error record written by kernels whose bounded waits gave up:
 // [0] = code (0 = none), [1] = kernel id, [2] = detail (barrier / stage).
 enum DeviceErr : int { kErrNone = 0, kErrWaitTimeout = 1 };
-enum KernelId : int { kKConvTc = 1, kKGnSlab = 2, kKDepthwise = 3, kKWaitProbe = 4 };
+enum KernelId : int { kKConvTc = 1, kKGnSlab = 2, kKDepthwise = 3, kKWaitProbe = 4, kKAttention = 5 };
 
 // Stream-ordered best-fit caching allocator (device analogue of the
 // reference's Scratch pool). All blocks are used on the context stream, so a
@@ -144,6 +144,9 @@ int64_t conv_gn_part_floats(const ConvShape& s, int64_t c_out);
 // that launch_gn_finalize takes (f32 per channel and chunk, then f64 over the group's channels).
 void launch_gn_fold_tiles(mbx_ctx* ctx, const float* tile_part, int64_t n, int64_t hw, int64_t c, int64_t groups,
                           double* part);
+// A tiled TMA map over 16-bit data (reads outside fill with zeros), 128-byte swizzle.
+void encode_tensor_map_16(CUtensorMap* map, const void* base, bool bf16, int rank, const uint64_t* dims,
+                          const uint64_t* strides, const uint32_t* box);
 // A tiled TMA map over f32 data: dims innermost first, strides in bytes for dims 1.., box in
 // elements; reads outside the map fill with zeros.
 void encode_tensor_map_f32(CUtensorMap* map, const float* base, int rank, const uint64_t* dims,
