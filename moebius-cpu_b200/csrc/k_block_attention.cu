@@ -147,7 +147,7 @@ constexpr int kRowsR = 4;
 constexpr int64_t kSms = 148;
 
 // Which kernel takes a problem, and over how many CTAs a list is split: enough to fill the card
-// twice over, never more than there are blocks (rows) or tiles of 128 keys (tensor cores).
+// twice over, never more than there are blocks (rows) or tiles of 64 keys (tensor cores).
 struct Plan {
     bool rows;
     int splits;
@@ -159,7 +159,7 @@ Plan plan_of(const BlockShape& s, int64_t topk) {
     p.rows = s.dtype == MBX_DTYPE_F32 && s.nq < 16;
     const int64_t tile = p.rows ? kRowsR : MBX_ATTENTION_BLOCK_Q;
     const int64_t ctas = std::max<int64_t>(1, s.n * s.heads * ((s.nq + tile - 1) / tile));
-    const int64_t pieces = p.rows ? topk : (topk * s.block_k + 127) / 128;
+    const int64_t pieces = p.rows ? topk : (topk * s.block_k + 63) / 64;
     p.splits = (int)std::max<int64_t>(1, std::min({(2 * kSms + ctas - 1) / ctas, pieces, int64_t(64)}));
     if (p.splits > 1)
         p.part_bytes = align256(sizeof(float) * (size_t)(s.n * s.nq * s.heads) * p.splits * (s.dim + 2));

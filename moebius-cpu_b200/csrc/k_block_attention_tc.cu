@@ -2,17 +2,20 @@
 // TMA-fed operands).
 //
 // A CTA takes one query block (128 rows) of one (item, head), or a share of its list, and walks
-// the listed key blocks in tiles of 128 keys (128 / block_k blocks a tile, each its own TMA box,
-// so any block size feeds the same tile). Six warps:
+// the listed key blocks in tiles of 64 keys (a part of a block, or several blocks with a TMA box
+// each, so any block size feeds the same tile). Six warps:
 //   warps 0-3  softmax: a thread owns a query row (a TMEM lane). It reads S from TMEM, keeps the
 //              running maximum and sum in f32 registers and writes the weights 2^(c·s − c·m)
 //              back over S, as the second product's left operand.
 //   warp 4     producer: TMA for Q once and for K, V of every tile; the tile's bits of valid keys.
 //   warp 5     MMA issuer (one thread) and TMEM allocation.
-// TMEM (256 columns): S, then P, in columns 0-127, O behind. Shared memory: Q, K and V in
-// 128-byte-swizzled panels of 64 channels; V serves as the N-major operand as it lies, so nothing
-// is transposed. Two CTAs share an SM (one for f32 with more than 64 channels): while one computes
-// weights, the other's products run.
+// TMEM: two S tiles of 64 columns, two P tiles (16-bit, up to 64 channels; else P lies over its S)
+// and O. While the weights of one tile are computed, Q·Kᵀ of the next runs into the other, so the softmax warps work back to back,
+// and two CTAs share an SM (one for f32 with more than 64 channels). 64 keys and not 128: two S
+// tiles of 128 columns and O would leave one CTA an SM; the price is Q·Kᵀ at N = 64, where reading
+// Q from shared memory takes 1.5 times the product's own cycles.
+// Shared memory: Q, K and V in 128-byte-swizzled panels of 64 channels; V serves as the N-major
+// operand as it lies, so nothing is transposed.
 //
 // 16-bit operands: P is rounded to their type (half a step of a weight, beside half a step of the
 // result at the end). The weights are relative to a reference that is raised only when a row's
@@ -24,7 +27,8 @@
 // 2^-39 of the largest. Three products (lo·hi, hi·lo, hi·hi; lo·lo is 2^-22 of the whole), and the
 // weights in two parts after a scale of 2^13. The tensor core truncates as it adds into its f32
 // accumulator, so a long sum there drifts by about 2^-25 a step: each tile's P·V starts a fresh
-// accumulator and the softmax threads add it to f32 registers, rounding to nearest.
+// accumulator (two in turn) and the softmax threads add it to f32 registers, rounding to nearest,
+// after they have handed over the next tile's weights.
 //
 // Masked keys: S becomes −inf; their V rows become zero in shared memory (16-bit) or while
 // splitting (f32), since zero times what a mask hides may be NaN.
@@ -41,12 +45,13 @@ namespace mbx {
 namespace {
 
 constexpr int kRows = MBX_ATTENTION_BLOCK_Q;
-constexpr int kKeys = 128;              // keys of a tile
-constexpr uint32_t kPanel = 128 * 128;  // bytes of 128 rows × 64 channels
+constexpr int kKeys = 64;                   // keys of a tile
+constexpr uint32_t kQPanel = kRows * 128;   // bytes of 64 channels of the query block
+constexpr uint32_t kPanel = kKeys * 128;    // and of a tile of K or V
 constexpr int kThreads = 192;
-constexpr uint32_t kTmemCols = 256;
-constexpr uint32_t kColO = 128;
-constexpr int kMaskSlots = 4;
+// Tiles whose bits of valid keys are kept: a slot is written again 8 tiles on, when Q·Kᵀ of 8 − stages tiles on is
+// complete, which was begun after P·V of two tiles before it, and so after this tile's bits were read (stages <= 6).
+constexpr int kMaskSlots = 8;
 constexpr float kLazy = 8.0f;    // log2 of the largest 16-bit weight
 constexpr int kScaleExp = 14;    // f32 operands: the largest magnitude becomes 2^14 .. 2^15
 constexpr int kWeightExp = 13;   // f32 operands: weights are scaled by 2^13
@@ -60,12 +65,26 @@ struct TcArgs {
 
 template <int PANELS, bool SPLIT>
 constexpr int stages_of() {
-    return !SPLIT && PANELS == 1 ? 2 : 1;
+    return !SPLIT && PANELS == 1 ? 4 : 2;
+}
+
+// TMEM: two S tiles; two P tiles of their own where that still leaves two CTAs an SM; O, two of them for f32.
+template <int PANELS, bool SPLIT>
+constexpr bool own_p() {
+    return PANELS == 1 && !SPLIT;
+}
+template <int PANELS, bool SPLIT>
+constexpr uint32_t col_o() {
+    return 2 * kKeys + (own_p<PANELS, SPLIT>() ? kKeys : 0);
+}
+template <int PANELS, bool SPLIT>
+constexpr uint32_t tmem_cols() {
+    return col_o<PANELS, SPLIT>() + PANELS * 64 * (SPLIT ? 2 : 1) <= 256 ? 256 : 512;
 }
 
 template <int PANELS, bool SPLIT>
 constexpr int smem_of() {
-    return (int)(PANELS * (SPLIT ? 2 : 1) * kPanel) * (1 + 2 * stages_of<PANELS, SPLIT>()) + 1024;
+    return PANELS * (SPLIT ? 2 : 1) * (int)(kQPanel + 2 * stages_of<PANELS, SPLIT>() * kPanel) + 1024;
 }
 
 // Columns of the warp's 32 lanes, complete on return: the wait is part of the statement, so that nothing that uses the
@@ -95,17 +114,14 @@ __device__ __forceinline__ void tmem_ld32_wait(uint32_t taddr, uint32_t (&r)[32]
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld128_wait(uint32_t taddr, uint32_t (&r)[128]) {
+__device__ __forceinline__ void tmem_ld64_wait(uint32_t taddr, uint32_t (&r)[64]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
         "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
         "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, "
         "%40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, "
-        "%59, %60, %61, %62, %63, %64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, "
-        "%78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, "
-        "%97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, "
-        "%113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127 "
-        "}, [%128];\n\t"
+        "%59, %60, %61, %62, %63 "
+        "}, [%64];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
@@ -114,16 +130,7 @@ __device__ __forceinline__ void tmem_ld128_wait(uint32_t taddr, uint32_t (&r)[12
           "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
           "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
           "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]),
-          "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]),
-          "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]),
-          "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]),
-          "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
         : "r"(taddr)
         : "memory");
 }
@@ -191,6 +198,13 @@ __device__ __forceinline__ void mma_16_ts(uint32_t d, uint32_t a, uint64_t bd, u
         : "memory");
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 template <class OUT>
 constexpr bool is_f32() {
     return std::is_same<OUT, float>::value;
@@ -205,29 +219,33 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
     constexpr bool BF16 = std::is_same<OUT, __nv_bfloat16>::value;
     constexpr int PLANES = SPLIT ? 2 : 1;
     constexpr int STAGES = stages_of<PANELS, SPLIT>();
-    constexpr uint32_t OP = PANELS * PLANES * kPanel;  // bytes of one operand's tile
+    constexpr uint32_t OP = PANELS * PLANES * kPanel;  // bytes of a tile of K or V
+    constexpr uint32_t TMEM = tmem_cols<PANELS, SPLIT>(), kColO = col_o<PANELS, SPLIT>();
+    constexpr bool OWN_P = own_p<PANELS, SPLIT>();
+    constexpr uint32_t PCOL = OWN_P ? 2 * kKeys : 0, PSTEP = OWN_P ? kKeys / 2 : kKeys;  // P tiles, else over S
     constexpr int DCOLS = PANELS * 64;
     using Part = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     const AttnArgs& a = args.a;
 
+    // Barriers that a tile in two uses come in pairs, one for the even tiles and one for the odd: a
+    // waiter is then never two phases behind, which a parity could not tell from none.
     enum {
         kKFull = 0,
         kKEmpty = kKFull + STAGES,
         kVFull = kKEmpty + STAGES,
         kVEmpty = kVFull + STAGES,
         kVClean = kVEmpty + STAGES,
-        kMFull = kVClean + STAGES,
-        kMEmpty = kMFull + kMaskSlots,
-        kQFull = kMEmpty + kMaskSlots,
-        kSFull,
-        kPFull,
-        kOFull,
-        kFin,
+        kQFull = kVClean + STAGES,
+        kSFull,               // [2] a tile's S is complete
+        kPFull = kSFull + 2,  // [2] a tile's weights are written
+        kOFull = kPFull + 2,   // [2] a tile's P·V is complete
+        kOEmpty = kOFull + 2,  // [2] f32: a tile's product is added to the registers
+        kFin = kOEmpty + 2,
         kBars
     };
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[kBars];
-    __shared__ uint32_t valid[kMaskSlots][4];
+    __shared__ volatile uint32_t valid[kMaskSlots][2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, listed;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -252,14 +270,14 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             mbar_init(bar(kKFull + i), 1), mbar_init(bar(kKEmpty + i), 1);
             mbar_init(bar(kVFull + i), 1), mbar_init(bar(kVEmpty + i), 1), mbar_init(bar(kVClean + i), 1);
         }
-        for (int i = 0; i < kMaskSlots; ++i) mbar_init(bar(kMFull + i), 1), mbar_init(bar(kMEmpty + i), 4);
-        mbar_init(bar(kQFull), 1), mbar_init(bar(kSFull), 1), mbar_init(bar(kPFull), 128);
-        mbar_init(bar(kOFull), 1), mbar_init(bar(kFin), 1);
+        for (int i = 0; i < 2; ++i) mbar_init(bar(kSFull + i), 2), mbar_init(bar(kPFull + i), 128);
+        for (int i = 0; i < 2; ++i) mbar_init(bar(kOFull + i), 1), mbar_init(bar(kOEmpty + i), 128);
+        mbar_init(bar(kQFull), 1), mbar_init(bar(kFin), 1);
         abort_flag = 0, listed = 0;
         fence_mbarrier_init();
     }
     if (warp == 5) {
-        tmem_alloc(smem_u32(&tmem_slot), kTmemCols);
+        tmem_alloc(smem_u32(&tmem_slot), TMEM);
         tmem_relinquish();
     }
     __syncthreads();
@@ -274,8 +292,8 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const int per_tile = kKeys / a.block_k;
-    const int all_tiles = (listed + per_tile - 1) / per_tile;
+    const int rows_box = min(a.block_k, kKeys), boxes = kKeys / rows_box;  // TMA boxes of a tile
+    const int all_tiles = (int)(((int64_t)listed * a.block_k + kKeys - 1) / kKeys);
     const int t0 = (int)((int64_t)all_tiles * split / a.splits);
     const int tiles = (int)((int64_t)all_tiles * (split + 1) / a.splits) - t0;
     volatile int* abort_p = &abort_flag;
@@ -303,64 +321,49 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         float acc[SPLIT ? DCOLS : 1];
 #pragma unroll
         for (int i = 0; i < (SPLIT ? DCOLS : 1); ++i) acc[i] = 0.0f;
-        auto fold = [&] {  // f32: the last tile's product joins the row's sum
+        // f32: adds the product of tile t, and brings the sum to the reference that holds since, 2^f lower.
+        auto fold = [&](int t, float f) {
 #pragma unroll
             for (int i = 0; i < (SPLIT ? DCOLS : 0); i += 32) {
                 uint32_t o[32];
-                tmem_ld32_wait(lanes + kColO + i, o);
+                tmem_ld32_wait(lanes + kColO + (t & 1) * DCOLS + i, o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) acc[SPLIT ? i + e : 0] += __uint_as_float(o[e]);
+                for (int e = 0; e < 32; ++e)
+                    acc[SPLIT ? i + e : 0] = (acc[SPLIT ? i + e : 0] + __uint_as_float(o[e])) * f;
             }
         };
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
             const int slot = j % kMaskSlots;
-            ok = warp_wait(kMFull + slot, j / kMaskSlots, 20);
-            if (!ok) break;
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = *(volatile uint32_t*)&valid[slot][i];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(kMEmpty + slot));
-            const bool full = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu;
-            ok = warp_wait(kSFull, j, 21);  // this tile's S; the last tile's P·V was complete before it was begun
+            const uint32_t sp = lanes + (j & 1) * kKeys, pp = lanes + PCOL + (j & 1) * PSTEP;  // its S and P
+            ok = warp_wait(kSFull + (j & 1), j >> 1, 21);
             if (!ok) break;
             tc_fence_after();
-            if (SPLIT && j > 0) fold();
-            constexpr int CH = SPLIT ? 32 : 128;  // columns in registers at a time
-            uint32_t s[CH];
-            float top = -INFINITY;
-            auto load = [&](int q) {
-                if constexpr (SPLIT)
-                    tmem_ld32_wait(lanes + q * CH, s);
-                else
-                    tmem_ld128_wait(lanes, s);
-                if (!full) {
+            const uint32_t w0 = valid[slot][0], w1 = valid[slot][1];
+            uint32_t s[kKeys];
+            tmem_ld64_wait(sp, s);
+            if ((w0 & w1) != 0xffffffffu) {
 #pragma unroll
-                    for (int i = 0; i < CH; ++i) {
-                        const uint32_t word = CH == 128 ? w[i >> 5] : (q == 0 ? w[0] : q == 1 ? w[1] : q == 2 ? w[2] : w[3]);
-                        if (!(word >> (i & 31) & 1u)) s[i] = 0xff800000u;
-                    }
-                }
-            };
-#pragma unroll
-            for (int q = 0; q < 128 / CH; ++q) {
-                load(q);
-                float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < CH; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(s[i]));
-                top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+                for (int i = 0; i < kKeys; ++i)
+                    if (!((i < 32 ? w0 : w1) >> (i & 31) & 1u)) s[i] = 0xff800000u;
             }
+            float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(s[i]));
+            const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
             // Raise the reference: to every new maximum (f32), or when a weight would pass 2^8.
             const bool raise = SPLIT || ref == -INFINITY ? top > ref : (top - ref) * c > kLazy;
+            float f = 1.0f;
             if (__any_sync(0xffffffffu, raise)) {
-                const float f = !raise ? 1.0f : (ref == -INFINITY ? 0.0f : ex2((ref - top) * c));
-                if (raise) ref = top;
+                if (raise) {
+                    f = ref == -INFINITY ? 0.0f : ex2((ref - top) * c);
+                    ref = top;
+                }
                 l *= f;
-                if (SPLIT) {
-#pragma unroll
-                    for (int i = 0; i < (SPLIT ? DCOLS : 0); ++i) acc[SPLIT ? i : 0] *= f;
-                } else if (j > 0) {
+                if (!SPLIT && j > 0) {
+                    ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 22);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll
                     for (int i = 0; i < DCOLS; i += 16) {
                         uint32_t o[16];
@@ -374,14 +377,12 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             const float mc = (ref == -INFINITY ? 0.0f : ref) * c - (SPLIT ? (float)kWeightExp : 0.0f);
             float sum[4] = {};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {  // 32 keys: 16 columns of P, and at f32 16 more of its low part
-                if (SPLIT) load(q);
+            for (int q = 0; q < kKeys / 32; ++q) {  // 32 keys: 16 columns of P, and for f32 16 more of its low part
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int at = (SPLIT ? 0 : q * 32) + 2 * i;
-                    const float p0 = ex2(fmaf(__uint_as_float(s[at]), c, -mc));
-                    const float p1 = ex2(fmaf(__uint_as_float(s[at + 1]), c, -mc));
+                    const float p0 = ex2(fmaf(__uint_as_float(s[q * 32 + 2 * i]), c, -mc));
+                    const float p1 = ex2(fmaf(__uint_as_float(s[q * 32 + 2 * i + 1]), c, -mc));
                     sum[i & 1] += p0, sum[2 + (i & 1)] += p1;
                     hi[i] = pack2(p0, p1, Part());
                     if (SPLIT) {
@@ -389,22 +390,29 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                         lo[i] = pack2(p0 - b.x, p1 - b.y, Part());
                     }
                 }
-                // f32 parts lie over their own 32 columns of S, whose other columns are still to be read.
-                tmem_st16_u32(lanes + q * (SPLIT ? 32 : 16), hi);
-                if (SPLIT) tmem_st16_u32(lanes + q * 32 + 16, lo);
+                tmem_st16_u32(pp + q * 16, hi);
+                if (SPLIT) tmem_st16_u32(pp + kKeys / 2 + q * 16, lo);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(bar(kPFull));
+            mbar_arrive(bar(kPFull + (j & 1)));
+            if (SPLIT && j > 0) {
+                ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 22);
+                if (!ok) break;
+                tc_fence_after();
+                fold(j - 1, f);
+                tc_fence_before();
+                mbar_arrive(bar(kOEmpty + ((j - 1) & 1)));
+            }
         }
-        if (ok && tiles > 0) ok = warp_wait(kOFull, tiles - 1, 22);
+        if (ok && tiles > 0) ok = warp_wait(kOFull + ((tiles - 1) & 1), (tiles - 1) >> 1, 35);
         if (ok) {
             tc_fence_after();
             const int64_t row = (int64_t)qb * kRows + warp * 32 + lane;
             const bool store = row < a.nq;
             const int64_t at = ((int64_t)item * a.nq + row) * a.heads + h;
-            if (SPLIT && tiles > 0) fold();
+            if (SPLIT && tiles > 0) fold(tiles - 1, 1.0f);
             // One factor for the row: 1 / l, or for a share of the list the weights' own scale taken out.
             const float f = a.splits > 1 ? (SPLIT ? ldexpf(1.0f, -ev - kWeightExp) : 1.0f)
                                          : (l == 0.0f ? 0.0f : (SPLIT ? ldexpf(1.0f, -ev) : 1.0f) / l);
@@ -437,53 +445,80 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         }
     } else if (warp == 4) {
         // ---------------------------------------------------------------- producer
-        auto load_tile = [&](const CUtensorMap* map, uint32_t dst, int full_bar, int head, int token, int boxes,
-                             int rows) {  // `boxes` lanes bring `rows` rows each
-            if (lane == 0) mbar_arrive_expect_tx(bar(full_bar), OP);
+        auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bytes, int full_bar, int head, int token,
+                        int n_boxes, int rows) {  // one lane for each box of `rows` rows
+            if (lane == 0) mbar_arrive_expect_tx(bar(full_bar), bytes);
             __syncwarp();
-            if (lane < boxes) {
+            if (lane < n_boxes) {
 #pragma unroll
                 for (int p = 0; p < PLANES * PANELS; ++p)
-                    tma_load_4d(dst + p * kPanel + lane * rows * 128, map, (p % PANELS) * 64, head, token,
-                                item + (p / PANELS) * (int)args.n, bar(full_bar));
+                    tma_load_4d(dst + p * (bytes / (PLANES * PANELS)) + lane * rows * 128, map, (p % PANELS) * 64, head,
+                                token, item + (p / PANELS) * (int)args.n, bar(full_bar));
             }
             __syncwarp();
         };
         int q_done = 0, k_done = 0, v_done = 0;
         if (tiles > 0) {
-            load_tile(&map_q, sq, kQFull, h, qb * kRows, 1, kRows);
+            load(&map_q, sq, PANELS * PLANES * kQPanel, kQFull, h, qb * kRows, 1, kRows);
             q_done = 1;
         }
+        // The list and the mask are read ahead of the tiles that they are for: a lane holds the first token of one
+        // box (32 / boxes tiles at a time, the next ones on their way), and its two keys' mask bytes of the next tile.
+        const int lg_block = 31 - __clz(a.block_k), lg_rows = 31 - __clz(rows_box), lg_boxes = 31 - __clz(boxes);
+        const int batch = 32 >> lg_boxes;
+        auto first_token = [&](int tile) {  // of this lane's box in the batch that begins with `tile`
+            const int at = (t0 + tile) * kKeys + (lane << lg_rows), e = at >> lg_block;  // in the list's keys
+            const int blk = e < listed ? list[e] : -1;
+            return (uint32_t)blk < (uint32_t)a.k_blocks ? (blk << lg_block) + (at & (a.block_k - 1))
+                                                        : (int)a.nk;  // past the last key: zeros
+        };
+        auto cut = [&](int t) {  // the batch's boxes with a key past the last one
+            return __ballot_sync(0xffffffffu, (int64_t)t + rows_box > a.nk);
+        };
+        int tokens = first_token(0), tokens_next = tiles > batch ? first_token(batch) : 0;
+        uint32_t short_boxes = cut(tokens);
+        const uint32_t box_bits = boxes == 1 ? 1u : boxes == 2 ? 3u : 15u;
+        uint8_t keep[2] = {1, 1};
+        int64_t t_key[2] = {0, 0};
+        bool checks = false;  // the tile's keys are looked at one by one
+        auto look_up = [&](int j) {
+            const int box0 = (j & (batch - 1)) << lg_boxes;
+            checks = mask || (short_boxes >> box0 & box_bits);
+            if (!checks) return;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int key = i * 32 + lane;
+                t_key[i] = (int64_t)__shfl_sync(0xffffffffu, tokens, box0 + (key >> lg_rows)) + (key & (rows_box - 1));
+                if (mask) keep[i] = t_key[i] < a.nk ? mask[t_key[i]] : 0;
+            }
+        };
+        if (tiles > 0) look_up(0);
         for (int j = 0; j < tiles; ++j) {
             const int st = j % STAGES, ph = j / STAGES, slot = j % kMaskSlots;
-            int token = (int)a.nk;  // past the last key: zeros
-            if (lane < per_tile) {
-                const int e = (t0 + j) * per_tile + lane;
-                const int blk = e < listed ? list[e] : -1;
-                if ((uint32_t)blk < (uint32_t)a.k_blocks) token = blk * a.block_k;
+            const int token = __shfl_sync(0xffffffffu, tokens, ((j & (batch - 1)) << lg_boxes) + (lane & (boxes - 1)));
+            uint32_t w[2] = {0xffffffffu, 0xffffffffu};
+            bool hidden = false;
+            if (checks) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bool in = t_key[i] < a.nk, kept = in && keep[i];
+                    w[i] = __ballot_sync(0xffffffffu, kept);
+                    hidden |= in && !kept;
+                }
+                hidden = __any_sync(0xffffffffu, hidden);
             }
             if (j >= STAGES && !warp_wait(kKEmpty + st, ph - 1, 23)) break;
-            load_tile(&map_k, sk + st * OP, kKFull + st, kh, token, per_tile, a.block_k);
+            if (lane == 0) valid[slot][0] = w[0], valid[slot][1] = w[1];  // handed on with K, then with S
+            load(&map_k, sk + st * OP, OP, kKFull + st, kh, token, boxes, rows_box);
             k_done = j + 1;
-            if (j >= kMaskSlots && !warp_wait(kMEmpty + slot, j / kMaskSlots - 1, 24)) break;
-            uint32_t w[4];
-            bool hidden = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = i * 32 + lane;
-                const int64_t t = (int64_t)__shfl_sync(0xffffffffu, token, key / a.block_k) + key % a.block_k;
-                const bool in = t < a.nk, keep = in && (!mask || mask[t]);
-                w[i] = __ballot_sync(0xffffffffu, keep);
-                hidden |= in && !keep;
+            if (((j + 1) & (batch - 1)) == 0) {
+                tokens = tokens_next;
+                short_boxes = cut(tokens);
+                if (j + 1 + batch < tiles) tokens_next = first_token(j + 1 + batch);
             }
-            hidden = __any_sync(0xffffffffu, hidden);
-            if (lane == 0) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) *(volatile uint32_t*)&valid[slot][i] = w[i];
-                mbar_arrive(bar(kMFull + slot));
-            }
+            if (j + 1 < tiles) look_up(j + 1);
             if (j >= STAGES && !warp_wait(kVEmpty + st, ph - 1, 25)) break;
-            load_tile(&map_v, sv + st * OP, kVFull + st, kh, token, per_tile, a.block_k);
+            load(&map_v, sv + st * OP, OP, kVFull + st, kh, token, boxes, rows_box);
             v_done = j + 1;
             if (cleans) {
                 if (hidden) {
@@ -509,60 +544,76 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             for (int i = std::max(0, v_done - STAGES); i < v_done; ++i)
                 drain_wait(bar(kVFull + i % STAGES), (uint32_t)(i / STAGES) & 1u, deadline, args.err, 27, kKAttention);
         }
-    } else if (lane == 0 && tiles > 0) {
+    } else if (tiles > 0) {
         // ---------------------------------------------------------------- MMA issuer
+        // The whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues.
+        const bool leader = elect_one();
         const int k_steps = (a.dim + 15) / 16;
         const uint32_t idesc_s = idesc_16(BF16, kKeys, a.scale < 0.0f, false);
         const uint32_t idesc_o = idesc_16(BF16, k_steps * 16, false, true);
-        bool ok = wait(kQFull, 0, 28);
+        const uint64_t q_desc = sw128_desc(sq), k_desc = sw128_desc(sk), v_desc = sw128_desc_mn(sv);
+        auto scores = [&](int j) {  // S of tile j, whose columns held S (and where P has none of its own, P) of tile j − 2
+            const int st = j % STAGES;
+            if (!warp_wait(kKFull + st, j / STAGES, 29)) return false;
+            if (!OWN_P && j >= 2 && !warp_wait(kOFull + (j & 1), (j - 2) >> 1, 30)) return false;
+            tc_fence_after();
+            if (leader) {
+#pragma unroll
+                for (int p = SPLIT ? 0 : 2; p < 3; ++p) {  // lo·hi, hi·lo, hi·hi
+                    const uint64_t qa = q_desc + (p == 0 ? PANELS * kQPanel >> 4 : 0);
+                    const uint64_t ka = k_desc + ((uint32_t)st * OP >> 4) + (p == 1 ? PANELS * kPanel >> 4 : 0);
+#pragma unroll
+                    for (int s = 0; s < 4 * PANELS; ++s)
+                        if (s < k_steps)
+                            mma_16_ss(tmem + (j & 1) * kKeys, qa + ((s >> 2) * kQPanel + (s & 3) * 32 >> 4),
+                                      ka + ((s >> 2) * kPanel + (s & 3) * 32 >> 4), idesc_s,
+                                      (p > (SPLIT ? 0 : 2) || s > 0) ? 1u : 0u);
+                }
+                mma_commit(bar(kKEmpty + st));
+                mma_commit(bar(kSFull + (j & 1)));
+                mbar_arrive(bar(kSFull + (j & 1)));  // the producer's bits of valid keys, seen here, go on with S
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = warp_wait(kQFull, 0, 28) && scores(0) && (tiles == 1 || scores(1));
         for (int j = 0; ok && j < tiles; ++j) {
             const int st = j % STAGES, ph = j / STAGES;
-            ok = wait(kKFull + st, ph, 29);
-            // S lies over the P that the last tile's product reads.
-            if (ok && j > 0) ok = wait(kOFull, j - 1, 30);
+            ok = warp_wait(kPFull + (j & 1), j >> 1, 33);
+            if (ok && OWN_P && j + 2 < tiles) ok = scores(j + 2);  // tile j's S was read before its P was written
+            if (ok) ok = warp_wait(kVFull + st, ph, 31);
+            if (ok && cleans) ok = warp_wait(kVClean + st, ph, 32);
+            if (ok && SPLIT && j >= 2) ok = warp_wait(kOEmpty + (j & 1), (j - 2) >> 1, 36);
             if (!ok) break;
             tc_fence_after();
+            if (leader) {
 #pragma unroll
-            for (int p = SPLIT ? 0 : 2; p < 3; ++p) {  // lo·hi, hi·lo, hi·hi
-                const uint32_t qa = sq + (p == 0 ? PANELS * kPanel : 0);
-                const uint32_t ka = sk + st * OP + (p == 1 ? PANELS * kPanel : 0);
-                for (int s = 0; s < k_steps; ++s) {
-                    const uint32_t off = (uint32_t)(s >> 2) * kPanel + (uint32_t)(s & 3) * 32u;
-                    mma_16_ss(tmem, sw128_desc(qa + off), sw128_desc(ka + off), idesc_s,
-                              (p > (SPLIT ? 0 : 2) || s > 0) ? 1u : 0u);
+                for (int p = SPLIT ? 0 : 2; p < 3; ++p) {
+                    const uint64_t va = v_desc + ((uint32_t)st * OP >> 4) + (p == 1 ? PANELS * kPanel >> 4 : 0);
+                    const uint32_t pa = tmem + PCOL + (j & 1) * PSTEP + (p == 0 ? kKeys / 2 : 0);
+#pragma unroll
+                    for (int s = 0; s < kKeys / 16; ++s) {
+                        const bool fresh = s == 0 && (SPLIT ? p == 0 : j == 0);
+                        mma_16_ts(tmem + kColO + (SPLIT ? (j & 1) * DCOLS : 0), pa + (uint32_t)s * 8u,
+                                  va + (uint32_t)(s * 2048 >> 4), idesc_o, fresh ? 0u : 1u);
+                    }
                 }
+                mma_commit(bar(kVEmpty + st));
+                mma_commit(bar(kOFull + (j & 1)));
             }
-            mma_commit(bar(kKEmpty + st));
-            mma_commit(bar(kSFull));
-            ok = wait(kVFull + st, ph, 31);
-            if (ok && cleans) ok = wait(kVClean + st, ph, 32);
-            if (ok) ok = wait(kPFull, j, 33);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int p = SPLIT ? 0 : 2; p < 3; ++p) {
-                const uint32_t va = sv + st * OP + (p == 1 ? PANELS * kPanel : 0);
-#pragma unroll
-                for (int s = 0; s < kKeys / 16; ++s) {
-                    const uint32_t pa = SPLIT ? (uint32_t)(s >> 1) * 32u + (uint32_t)(s & 1) * 8u + (p == 0 ? 16u : 0u)
-                                              : (uint32_t)s * 8u;
-                    const bool fresh = s == 0 && (SPLIT ? p == 0 : j == 0);
-                    mma_16_ts(tmem + kColO, tmem + pa, sw128_desc_mn(va + (uint32_t)s * 2048u), idesc_o,
-                              fresh ? 0u : 1u);
-                }
-            }
-            mma_commit(bar(kVEmpty + st));
-            mma_commit(bar(kOFull));
+            __syncwarp();
+            if (!OWN_P && j + 2 < tiles) ok = scores(j + 2);
         }
-        if (!ok) {  // MMAs in flight finish before TMEM is freed
+        if (!ok && leader) {  // MMAs in flight finish before TMEM is freed
             mma_commit(bar(kFin));
             drain_wait(bar(kFin), 0, clock64() + kWaitLimit, args.err, 34, kKAttention);
         }
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 5) tmem_dealloc(tmem, kTmemCols);
+    if (warp == 5) tmem_dealloc(tmem, TMEM);
 }
 
 // ------------------------------------------------------------------------------------ f32 operands
@@ -691,7 +742,7 @@ void launch_attention_tc(mbx_ctx* ctx, const AttnArgs& a, int dtype, int64_t n, 
     CUtensorMap maps[3];
     for (int i = 0; i < 3; ++i)
         encode_heads(&maps[i], x[i], dtype == MBX_DTYPE_BF16, planes * n, rows[i], heads[i], a.dim, stride[i],
-                     i == 0 ? kRows : a.block_k);
+                     i == 0 ? kRows : std::min(a.block_k, kKeys));
     if (dtype == MBX_DTYPE_F32) return a.dim > 64 ? launch_typed<float, 2>(ctx, t, maps) : launch_typed<float, 1>(ctx, t, maps);
     if (dtype == MBX_DTYPE_F16) return a.dim > 64 ? launch_typed<__half, 2>(ctx, t, maps) : launch_typed<__half, 1>(ctx, t, maps);
     a.dim > 64 ? launch_typed<__nv_bfloat16, 2>(ctx, t, maps) : launch_typed<__nv_bfloat16, 1>(ctx, t, maps);
