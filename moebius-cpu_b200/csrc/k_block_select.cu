@@ -19,6 +19,8 @@
 //  * block_topk: a warp per row of scores, its keys in registers: the topk-th
 //    largest is found by bisection, counting the keys at or above a candidate,
 //    and the survivors are written by prefix counts.
+#include <algorithm>
+
 #include "mbx_device.cuh"
 #include "mbx_internal.h"
 
@@ -31,75 +33,84 @@ struct MeanSide {
     const void* x;
     int64_t x_stride, rows;    // elements between rows; rows of an item
     int block, blocks;         // rows of a block, blocks of an item
-    int chunks, cols, groups;  // 8-channel chunks of a row; those of one CTA; CTAs of a block
+    int width, cols, groups;   // channels of a row; 16-byte pieces of it a CTA takes; CTAs of a block
     const uint8_t* mask;       // [n][rows] or null
-    double* mean;              // [n][blocks][chunks · 8]
+    double* mean;              // [n][blocks][width]
     uint8_t* live;             // [n][blocks]: 1 where a row was unmasked (null: not wanted)
 };
 
 struct MeanArgs {
     MeanSide side[2];  // q, k
-    int64_t first_k;   // CTAs before this one are q's
 };
 
+// Grid: (blocks of q, then of k; groups of columns; items). A thread adds a 16-byte piece of every
+// lanes-th row. It has a ring of kRing rows of its own in shared memory that cp.async fills, so that
+// up to 32 KB a CTA are on their way with few registers and nobody waits for another thread: with
+// register loads the conversions to f64 (an eighth of the f32 rate) and the loads took turns, at
+// 4.1 TB/s. Rows that the mask hides, or past the last one, are filled with zeros.
+constexpr int kRing = 8;
+
 template <class T>
-__global__ void __launch_bounds__(kMeanThreads) block_means_kernel(const __grid_constant__ MeanArgs args) {
-    __shared__ double part[kMeanThreads * 8];
-    __shared__ int count;
-    const bool is_k = blockIdx.x >= args.first_k;
+__global__ void __launch_bounds__(kMeanThreads, 5) block_means_kernel(const __grid_constant__ MeanArgs args) {
+    constexpr int E = 16 / sizeof(T);  // channels of a piece
+    __shared__ __align__(16) uint8_t ring[kRing * kMeanThreads * 16];
+    __shared__ uint8_t keep[MBX_ATTENTION_BLOCK_Q];
+    const bool is_k = (int)blockIdx.x >= args.side[0].blocks;
     const MeanSide& a = args.side[is_k];
-    const int64_t cta = blockIdx.x - (is_k ? args.first_k : 0);
-    const int group = (int)(cta % a.groups);
-    const int64_t at = cta / a.groups;  // item · blocks + block
-    const int64_t item = at / a.blocks, r0 = (at - item * a.blocks) * a.block;
+    if ((int)blockIdx.y >= a.groups) return;
+    const int blk = (int)blockIdx.x - (is_k ? args.side[0].blocks : 0);
+    const int64_t item = blockIdx.z, r0 = (int64_t)blk * a.block, at = item * a.blocks + blk;
     const int rows = (int)min((int64_t)a.block, a.rows - r0);
     const int lanes = kMeanThreads / a.cols, rl = threadIdx.x / a.cols, col = threadIdx.x - rl * a.cols;
-    const int chunk = group * a.cols + col;
-    const bool on = rl < lanes && chunk < a.chunks;
-    const T* x = static_cast<const T*>(a.x) + (item * a.rows + r0) * a.x_stride + (int64_t)chunk * 8;
-    const uint8_t* mask = a.mask ? a.mask + item * a.rows + r0 : nullptr;
-    if (threadIdx.x == 0) count = 0;
-    __syncthreads();
-    double sum[8] = {};
-    if (on) {
-        constexpr int U = sizeof(T) == 2 ? 8 : 4;  // rows in flight
-        typename Raw8<T>::type raw[U];
-        for (int r = rl; r < rows; r += U * lanes) {
-            bool keep[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int ru = r + u * lanes;
-                keep[u] = ru < rows && (!mask || mask[ru]);
-                if (keep[u]) raw[u] = load_raw8(x + ru * a.x_stride);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (!keep[u]) continue;
-                float v[8];
-                widen8<T>(raw[u], v);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i] += (double)v[i];
-            }
+    const int ch = (blockIdx.y * a.cols + col) * E;  // first channel
+    int count = rows;
+    if (a.mask) {
+        const uint8_t m = (int)threadIdx.x < rows ? a.mask[item * a.rows + r0 + threadIdx.x] : 0;
+        if (threadIdx.x < MBX_ATTENTION_BLOCK_Q) keep[threadIdx.x] = m;
+        count = __syncthreads_count(m != 0);
+    }
+    const T* x = static_cast<const T*>(a.x) + (item * a.rows + r0) * a.x_stride + ch;
+    const uint32_t slot0 = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
+    const int mine = rl < lanes && ch < a.width ? (rows - rl + lanes - 1) / lanes : 0;  // rows of this thread
+    auto request = [&](int i) {  // the i-th of them
+        if (i < mine) {
+            const int r = rl + i * lanes;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot0 + i % kRing * (kMeanThreads * 16)),
+                         "l"(x + r * a.x_stride), "r"(a.mask && !keep[r] ? 0 : 16)
+                         : "memory");
         }
-    }
-    if (mask) {
-        for (int r = threadIdx.x; r < rows; r += kMeanThreads)
-            if (mask[r]) atomicAdd(&count, 1);
-    } else if (threadIdx.x == 0) {
-        count = rows;
-    }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    double sum[E] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) part[i * kMeanThreads + threadIdx.x] = sum[i];
+    for (int i = 0; i < kRing; ++i) request(i);
+    for (int i = 0; i < mine; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+        const uint4 raw = *reinterpret_cast<const uint4*>(ring + (i % kRing * kMeanThreads + threadIdx.x) * 16);
+        float v[E];
+        if constexpr (E == 8) {
+            widen8<T>(raw, v);
+        } else {
+            v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y);
+            v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
+        }
+        request(i + kRing);
+#pragma unroll
+        for (int c = 0; c < E; ++c) sum[c] += (double)v[c];
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    const int n = count;
-    for (int e = threadIdx.x; e < a.cols * 8; e += kMeanThreads) {
-        const int c = e >> 3, i = e & 7;
+    double* part = reinterpret_cast<double*>(ring);  // at most 16 KB of its 32
+#pragma unroll
+    for (int i = 0; i < E; ++i) part[i * kMeanThreads + threadIdx.x] = sum[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.cols * E; e += kMeanThreads) {
+        const int c = e / E, i = e % E, to = (blockIdx.y * a.cols + c) * E + i;
         double s = 0.0;
         for (int w = 0; w < lanes; ++w) s += part[i * kMeanThreads + w * a.cols + c];
-        if (group * a.cols + c < a.chunks)
-            a.mean[(at * a.chunks + group * a.cols + c) * 8 + i] = s / (double)max(n, 1);
+        if (to < a.width) a.mean[at * a.width + to] = s / (double)max(count, 1);
     }
-    if (a.live && group == 0 && threadIdx.x == 0) a.live[at] = n > 0;
+    if (a.live && blockIdx.y == 0 && threadIdx.x == 0) a.live[at] = count > 0;
 }
 
 // An integer that orders as the score does: 0 for a block without an unmasked key (never chosen), then −inf … +inf,
@@ -111,10 +122,11 @@ __device__ __forceinline__ uint64_t order_key(double s, bool live) {
     return b < 0 ? ~(uint64_t)b : (uint64_t)b | (1ull << 63);
 }
 
-// keys[b][h][i][j] for a TI × TJ tile; 64 threads of (TI / 8) × (TJ / 8) outputs, kSK channels a step. The
-// wide tile gives 64 products for 16 values read from shared memory, which is what f64 arithmetic needs to
-// run at its rate; the narrow one spreads a small problem over more CTAs.
-constexpr int kSK = 16;
+// keys[b][h][i][j] for a 2·WI × 2·WJ tile, a WI × WJ part a warp, kSK channels a step. f64 products by mma.sync
+// (m16n8k4; f64 has no tcgen05 kind): eight values a lane from shared memory for 4096 products of a 32 × 32
+// part, where a 8 × 4 tile of plain FMAs reads 12 for 1024 and is bound by shared memory at 52 % of the f64 rate.
+// The small tile spreads a small problem over more CTAs.
+constexpr int kSK = 16, kScoreThreads = 128;
 
 struct ScoreArgs {
     const double *qm, *km;  // [n][q_blocks][heads][dim], [n][k_blocks][kv_heads][dim]
@@ -123,66 +135,90 @@ struct ScoreArgs {
     int heads, kv_heads, dim, q_blocks, k_blocks;
 };
 
-template <int TI, int TJ>
-__global__ void __launch_bounds__(64) block_scores_kernel(const ScoreArgs a) {
-    constexpr int RI = TI / 8, RJ = TJ / 8;
-    __shared__ double qs[2][kSK][TI + 1], ks[2][kSK][TJ + 1];
+__device__ __forceinline__ void mma_f64(double (&c)[4], const double (&a)[2], double b) {
+    asm("mma.sync.aligned.m16n8k4.row.col.f64.f64.f64.f64 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
+        : "+d"(c[0]), "+d"(c[1]), "+d"(c[2]), "+d"(c[3])
+        : "d"(a[0]), "d"(a[1]), "d"(b));
+}
+
+template <int WI, int WJ>
+__global__ void __launch_bounds__(kScoreThreads, 4) block_scores_kernel(const ScoreArgs a) {
+    constexpr int TI = 2 * WI, TJ = 2 * WJ, MI = WI / 16, NJ = WJ / 8;
+    // 20 values a row of 16: four channels of four rows fall into different banks.
+    constexpr int ROW = kSK + 4;
+    __shared__ __align__(16) double qs[2][TI][ROW], ks[2][TJ][ROW];
     const int64_t item = blockIdx.z / a.heads;
     const int h = blockIdx.z % a.heads, kh = h / (a.heads / a.kv_heads);
     const int i0 = blockIdx.y * TI, j0 = blockIdx.x * TJ;
-    const int tr = threadIdx.x / 8, tc = threadIdx.x % 8;
-    // A thread brings channel lc of rows lr, lr + 4, … of a step.
-    const int lc = threadIdx.x % kSK, lr = threadIdx.x / kSK;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int wi = (warp >> 1) * WI, wj = (warp & 1) * WJ, lr4 = lane >> 2, lc4 = lane & 3;
+    // A thread brings channels 2·lc, 2·lc + 1 of rows lr, lr + 16, … of a step; outside there are zeros.
+    const int lc = threadIdx.x % 8 * 2, lr = threadIdx.x / 8;
     const double* q = a.qm + (item * a.q_blocks * a.heads + h) * a.dim + lc;
     const double* k = a.km + (item * a.k_blocks * a.kv_heads + kh) * a.dim + lc;
     const int64_t q_row = (int64_t)a.heads * a.dim, k_row = (int64_t)a.kv_heads * a.dim;
-    double qr[TI / 4], kr[TJ / 4];
-    auto fetch = [&](int c0) {
+    auto copy = [](double* to, const double* from, bool in) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)),
+                     "l"(from), "r"(in ? 16 : 0)
+                     : "memory");
+    };
+    auto fetch = [&](int b, int c0) {
         const bool in = c0 + lc < a.dim;
 #pragma unroll
-        for (int r = 0; r < TI / 4; ++r) {
-            const int i = i0 + lr + 4 * r;
-            qr[r] = in && i < a.q_blocks ? q[i * q_row + c0] : 0.0;
+        for (int r = 0; r < TI / 16; ++r) {
+            const bool ok = in && i0 + lr + 16 * r < a.q_blocks;
+            copy(&qs[b][lr + 16 * r][lc], ok ? q + (i0 + lr + 16 * r) * q_row + c0 : a.qm, ok);
         }
 #pragma unroll
-        for (int r = 0; r < TJ / 4; ++r) {
-            const int j = j0 + lr + 4 * r;
-            kr[r] = in && j < a.k_blocks ? k[j * k_row + c0] : 0.0;
+        for (int r = 0; r < TJ / 16; ++r) {
+            const bool ok = in && j0 + lr + 16 * r < a.k_blocks;
+            copy(&ks[b][lr + 16 * r][lc], ok ? k + (j0 + lr + 16 * r) * k_row + c0 : a.km, ok);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    double acc[RI][RJ] = {};
-    fetch(0);
+    double acc[MI][NJ][4] = {};
+    fetch(0, 0);
     for (int c0 = 0, b = 0; c0 < a.dim; c0 += kSK, b ^= 1) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // this step is there, and everybody is done with the one before it
+        if (c0 + kSK < a.dim) fetch(b ^ 1, c0 + kSK);
 #pragma unroll
-        for (int r = 0; r < TI / 4; ++r) qs[b][lc][lr + 4 * r] = qr[r];
+        for (int c = 0; c < kSK; c += 4) {
+            double qv[MI][2], kv[NJ];
 #pragma unroll
-        for (int r = 0; r < TJ / 4; ++r) ks[b][lc][lr + 4 * r] = kr[r];
-        __syncthreads();
-        if (c0 + kSK < a.dim) fetch(c0 + kSK);
+            for (int r = 0; r < MI; ++r)
 #pragma unroll
-        for (int c = 0; c < kSK; ++c) {
-            double qv[RI], kv[RJ];
+                for (int e = 0; e < 2; ++e) qv[r][e] = qs[b][wi + r * 16 + e * 8 + lr4][c + lc4];
 #pragma unroll
-            for (int r = 0; r < RI; ++r) qv[r] = qs[b][c][tr + 8 * r];
+            for (int s = 0; s < NJ; ++s) kv[s] = ks[b][wj + s * 8 + lr4][c + lc4];
 #pragma unroll
-            for (int s = 0; s < RJ; ++s) kv[s] = ks[b][c][tc + 8 * s];
+            for (int r = 0; r < MI; ++r)
 #pragma unroll
-            for (int r = 0; r < RI; ++r)
-#pragma unroll
-                for (int s = 0; s < RJ; ++s) acc[r][s] = fma(qv[r], kv[s], acc[r][s]);
+                for (int s = 0; s < NJ; ++s) mma_f64(acc[r][s], qv[r], kv[s]);
         }
     }
 #pragma unroll
-    for (int s = 0; s < RJ; ++s) {
-        const int j = j0 + tc + 8 * s;
-        if (j >= a.k_blocks) continue;
-        const bool live = a.live[item * a.k_blocks + j] != 0;
+    for (int s = 0; s < NJ; ++s) {
+        const int j = j0 + wj + s * 8 + lc4 * 2;
+        bool live[2];
 #pragma unroll
-        for (int r = 0; r < RI; ++r) {
-            const int i = i0 + tr + 8 * r;
-            if (i < a.q_blocks) a.key[((int64_t)blockIdx.z * a.q_blocks + i) * a.k_blocks + j] = order_key(acc[r][s], live);
-        }
+        for (int e = 0; e < 2; ++e) live[e] = j + e < a.k_blocks && a.live[item * a.k_blocks + j + e] != 0;
+#pragma unroll
+        for (int r = 0; r < MI; ++r)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                const int i = i0 + wi + r * 16 + f * 8 + lr4;
+                if (i >= a.q_blocks) continue;
+                uint64_t* to = a.key + ((int64_t)blockIdx.z * a.q_blocks + i) * a.k_blocks + j;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (j + e < a.k_blocks) to[e] = order_key(acc[r][s][2 * f + e], live[e]);
+            }
     }
+}
+
+__device__ __forceinline__ double key_score(uint64_t key) {
+    return __longlong_as_double((int64_t)(key >> 63 ? key & ~(1ull << 63) : ~key));
 }
 
 constexpr int kTopWarps = 4;
@@ -200,46 +236,60 @@ __global__ void __launch_bounds__(kTopWarps * 32) block_topk_kernel(const uint64
     uint64_t mine[N > 0 ? N : 1];
 #pragma unroll
     for (int u = 0; u < N; ++u) mine[u] = u * 32 + lane < k_blocks ? s[u * 32 + lane] : 0;
+    auto for_each = [&](auto&& f) {
+        if constexpr (N > 0) {
+#pragma unroll
+            for (int u = 0; u < N; ++u) f(mine[u]);
+        } else {
+            for (int j = lane; j < k_blocks; j += 32) f(s[j]);
+        }
+    };
     auto count_at_least = [&](uint64_t t) {
         int c = 0;
-        if constexpr (N > 0) {
-#pragma unroll
-            for (int u = 0; u < N; ++u) c += mine[u] >= t;
-        } else {
-            for (int j = lane; j < k_blocks; j += 32) c += s[j] >= t;
-        }
+        for_each([&](uint64_t v) { c += v >= t; });
         return __reduce_add_sync(0xffffffffu, c);
     };
-    const int k = (int)min(topk, (int64_t)count_at_least(1));
-    // lo: the largest threshold known to leave k keys or more; at hi there are fewer.
-    uint64_t lo = 1, hi = ~0ull;
-    int at_least = k == 0 ? 0 : count_at_least(lo);
-    if (k > 0 && count_at_least(hi) >= k) lo = hi, at_least = count_at_least(lo);
-    if (at_least > k && lo != hi) {
-        // Narrow the range to the keys' own before halving it: scores share their leading bits.
-        uint64_t top = 0, low = ~0ull;
-        auto see = [&](uint64_t v) {
-            if (v == 0) return;
-            top = max(top, v), low = min(low, v);
-        };
-        if constexpr (N > 0) {
-#pragma unroll
-            for (int u = 0; u < N; ++u) see(mine[u]);
-        } else {
-            for (int j = lane; j < k_blocks; j += 32) see(s[j]);
-        }
-        for (int o = 16; o > 0; o >>= 1) {
-            top = max(top, (uint64_t)__shfl_xor_sync(0xffffffffu, top, o));
-            low = min(low, (uint64_t)__shfl_xor_sync(0xffffffffu, low, o));
-        }
-        lo = low, hi = top == ~0ull ? top : top + 1;
-        while (at_least != k && hi - lo > 1) {
-            const uint64_t mid = lo + (hi - lo) / 2;
-            const int c = count_at_least(mid);
+    // The high words' range (of the blocks that count) and how many there are.
+    uint32_t top = 0, low = ~0u;
+    int live = 0;
+    for_each([&](uint64_t v) {
+        const uint32_t w = (uint32_t)(v >> 32);
+        live += v != 0;
+        top = max(top, w);
+        if (v != 0) low = min(low, w);
+    });
+    live = __reduce_add_sync(0xffffffffu, live);
+    top = __reduce_max_sync(0xffffffffu, top);
+    low = __reduce_min_sync(0xffffffffu, low);
+    const int k = (int)min(topk, (int64_t)live);
+    // The largest threshold that k keys or more reach: on the high words, between the row's own extremes, and only
+    // where several keys share the last high word on the low ones.
+    uint64_t lo = 1;
+    int at_least = live;
+    if (k > 0 && live > k) {
+        // Halving the scores' range finds the place among scores of one magnitude in few steps, where the integers'
+        // range is mostly exponents that no score has; halving the integers' bounds the steps for any others.
+        uint64_t a32 = low, b32 = (uint64_t)top + 1;
+        for (int step = 0; at_least != k && b32 - a32 > 1; ++step) {
+            uint64_t mid = a32 + (b32 - a32) / 2;
+            if (step < 16) {
+                const uint64_t m = order_key(0.5 * key_score(a32 << 32) + 0.5 * key_score(b32 << 32), true) >> 32;
+                if (m > a32 && m < b32) mid = m;
+            }
+            int c = 0;
+            for_each([&](uint64_t v) { c += (uint32_t)(v >> 32) >= (uint32_t)mid; });
+            c = __reduce_add_sync(0xffffffffu, c);
             if (c >= k)
-                lo = mid, at_least = c;
+                a32 = mid, at_least = c;
             else
-                hi = mid;
+                b32 = mid;
+        }
+        lo = max(a32 << 32, (uint64_t)1);
+        uint64_t span = 1ull << 32;
+        while (at_least != k && span > 1) {
+            span /= 2;
+            const int c = count_at_least(lo + span);
+            if (c >= k) lo += span, at_least = c;
         }
     }
     // Above lo: all of them; equal to lo: the lowest blocks, as many as are still wanted.
@@ -269,17 +319,23 @@ __global__ void __launch_bounds__(kTopWarps * 32) block_topk_kernel(const uint64
 }
 
 template <class T>
-void launch_means(mbx_ctx* ctx, const MeanArgs& a, int64_t ctas) {
-    block_means_kernel<T><<<(unsigned)ctas, kMeanThreads, 0, ctx->stream>>>(a);
+void launch_means(mbx_ctx* ctx, const MeanArgs& a, int64_t n) {
+    const dim3 grid((unsigned)(a.side[0].blocks + a.side[1].blocks),
+                    (unsigned)std::max(a.side[0].groups, a.side[1].groups), (unsigned)n);
+    block_means_kernel<T><<<grid, kMeanThreads, 0, ctx->stream>>>(a);
     after_launch(ctx, "block_means");
 }
 
-MeanSide mean_side(const void* x, int64_t stride, int64_t rows, int block, int blocks, int64_t width,
-                   const uint8_t* mask, double* mean, uint8_t* live) {
-    MeanSide m{x, stride, rows, block, blocks, (int)(width / 8), 0, 0, mask, mean, live};
-    // At most 64 chunks a CTA (a KB of a 16-bit row), evenly: no group of few leftovers.
-    m.groups = (m.chunks + 63) / 64;
-    m.cols = (m.chunks + m.groups - 1) / m.groups;
+MeanSide mean_side(const void* x, int dtype, int64_t stride, int64_t rows, int block, int blocks, int64_t width,
+                   const uint8_t* mask, double* mean, uint8_t* live, int64_t n) {
+    MeanSide m{x, stride, rows, block, blocks, (int)width, 0, 0, mask, mean, live};
+    // 64 pieces (a KB) of a row for a CTA, evenly; 32 where that leaves fewer than four CTAs an SM. A CTA's fixed
+    // costs want long columns (65536 x 16 x 128 bf16: 217 us in all with 32, 202 with 64, 200 with 128), a small
+    // problem many CTAs (2 x 1961 and 4133 x 80 f32: 25 us with 32, 27 with 64, 34 with 128).
+    const int pieces = (int)width / (dtype == MBX_DTYPE_F32 ? 4 : 8);
+    const int most = n * blocks * ((pieces + 63) / 64) < 4 * 148 ? 32 : 64;
+    m.groups = (pieces + most - 1) / most;
+    m.cols = (pieces + m.groups - 1) / m.groups;
     return m;
 }
 
@@ -319,26 +375,23 @@ void launch_block_select(mbx_ctx* ctx, const BlockShape& s, const void* q, int64
     uint64_t* keys = reinterpret_cast<uint64_t*>(ws + l.key);
     if (kb > 0) {
         MeanArgs m{};
-        m.side[0] = mean_side(q, q_stride, s.nq, MBX_ATTENTION_BLOCK_Q, qb, s.heads * s.dim, nullptr,
-                              reinterpret_cast<double*>(ws + l.qm), nullptr);
-        m.side[1] = mean_side(k, k_stride, s.nk, (int)s.block_k, kb, s.kv_heads * s.dim, key_mask,
-                              reinterpret_cast<double*>(ws + l.km), ws + l.live);
-        m.first_k = s.n * qb * m.side[0].groups;
-        const int64_t ctas = m.first_k + s.n * kb * m.side[1].groups;
-        MBX_REQUIRE(ctas < (int64_t(1) << 31), "block_select: too many blocks");
+        m.side[0] = mean_side(q, s.dtype, q_stride, s.nq, MBX_ATTENTION_BLOCK_Q, qb, s.heads * s.dim, nullptr,
+                              reinterpret_cast<double*>(ws + l.qm), nullptr, s.n);
+        m.side[1] = mean_side(k, s.dtype, k_stride, s.nk, (int)s.block_k, kb, s.kv_heads * s.dim, key_mask,
+                              reinterpret_cast<double*>(ws + l.km), ws + l.live, s.n);
         if (s.dtype == MBX_DTYPE_F32)
-            launch_means<float>(ctx, m, ctas);
+            launch_means<float>(ctx, m, s.n);
         else if (s.dtype == MBX_DTYPE_F16)
-            launch_means<__half>(ctx, m, ctas);
+            launch_means<__half>(ctx, m, s.n);
         else
-            launch_means<__nv_bfloat16>(ctx, m, ctas);
+            launch_means<__nv_bfloat16>(ctx, m, s.n);
         ScoreArgs sc{m.side[0].mean, m.side[1].mean, ws + l.live, keys, (int)s.heads, (int)s.kv_heads, (int)s.dim, qb,
                      kb};
         const unsigned z = (unsigned)(s.n * s.heads);
         if ((int64_t)z * ((qb + 63) / 64) * ((kb + 63) / 64) >= 4 * (int64_t)ctx->sm_count)
-            block_scores_kernel<64, 64><<<dim3((kb + 63) / 64, (qb + 63) / 64, z), 64, 0, ctx->stream>>>(sc);
+            block_scores_kernel<32, 32><<<dim3((kb + 63) / 64, (qb + 63) / 64, z), kScoreThreads, 0, ctx->stream>>>(sc);
         else
-            block_scores_kernel<32, 32><<<dim3((kb + 31) / 32, (qb + 31) / 32, z), 64, 0, ctx->stream>>>(sc);
+            block_scores_kernel<16, 16><<<dim3((kb + 31) / 32, (qb + 31) / 32, z), kScoreThreads, 0, ctx->stream>>>(sc);
         after_launch(ctx, "block_scores");
     }
     const int64_t rows = s.n * s.heads * qb;
