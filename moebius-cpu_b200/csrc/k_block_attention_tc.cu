@@ -6,7 +6,7 @@
 // each, so any block size feeds the same tile). Six warps:
 //   warps 0-3  softmax: a thread owns a query row (a TMEM lane). It reads S from TMEM, keeps the
 //              running maximum and sum in f32 registers and writes the weights 2^(c·s − c·m)
-//              back over S, as the second product's left operand.
+//              back to TMEM, as the second product's left operand.
 //   warp 4     producer: TMA for Q once and for K, V of every tile; the tile's bits of valid keys.
 //   warp 5     MMA issuer (one thread) and TMEM allocation.
 // TMEM: two S tiles of 64 columns, two P tiles (16-bit, up to 64 channels; else P lies over its S)
@@ -22,10 +22,10 @@
 // maximum outgrows it by 2^8, so O, which accumulates in TMEM over the whole list, is rarely
 // rescaled.
 //
-// f32 operands: q, k and v are split beforehand into two f16 parts, after a power-of-two scale that
-// brings the largest magnitude of the head to 2^14: a value is held to 2^-22 of itself, or to
-// 2^-39 of the largest. Three products (lo·hi, hi·lo, hi·hi; lo·lo is 2^-22 of the whole), and the
-// weights in two parts after a scale of 2^13. The tensor core truncates as it adds into its f32
+// f32 operands: two f16 parts of every value after a power-of-two scale (k and v beforehand, by
+// head; a query row by the thread that owns it, as it begins): a value is held to 2^-23 of itself or of
+// the largest. Three products (lo·hi, hi·lo, hi·hi; lo·lo is 2^-22 of the whole), and the weights in
+// two parts after a scale of 2^7. The tensor core truncates as it adds into its f32
 // accumulator, so a long sum there drifts by about 2^-25 a step: each tile's P·V starts a fresh
 // accumulator (two in turn) and the softmax threads add it to f32 registers, rounding to nearest,
 // after they have handed over the next tile's weights.
@@ -52,13 +52,14 @@ constexpr int kThreads = 192;
 // Tiles whose bits of valid keys are kept: a slot is written again 8 tiles on, when Q·Kᵀ of 8 − stages tiles on is
 // complete, which was begun after P·V of two tiles before it, and so after this tile's bits were read (stages <= 6).
 constexpr int kMaskSlots = 8;
-constexpr float kLazy = 8.0f;    // log2 of the largest 16-bit weight
-constexpr int kScaleExp = 14;    // f32 operands: the largest magnitude becomes 2^14 .. 2^15
-constexpr int kWeightExp = 13;   // f32 operands: weights are scaled by 2^13
+constexpr float kLazy = 8.0f;   // log2 of the largest weight
+constexpr int kWeightExp = 7;   // f32 operands: weights are scaled by 2^7 before their split, up to 2^15
+constexpr int kScaleExp = 14;   // f32 operands: a scaled head's largest magnitude is in [2^14, 2^15)
+constexpr int kFixedExp = 6;    // and the exponent that most heads get, see attention_split_kernel
 
 struct TcArgs {
     AttnArgs a;
-    const uint32_t* amax;  // f32 operands: bits of the largest magnitudes, q [n][heads], k and v [n][kv_heads]
+    const uint32_t* amax;  // f32 operands: bits of the largest magnitudes, k and then v, [n][kv_heads] each
     int64_t n;
     int* err;
 };
@@ -158,10 +159,28 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The exponent of the power of two that scales a head whose largest magnitude has these bits.
+// The exponent of the power of two that scales values whose largest magnitude has these bits.
 __device__ __forceinline__ int scale_exponent(uint32_t bits) {
     if (bits == 0) return 0;
     return min(kScaleExp + 127 - max((int)(bits >> 23), 1), 126);
+}
+// kFixedExp fits a largest magnitude in [2^-8, 2^9): scaled, it is below 2^15, and the parts' absolute error of
+// 2^-25 is 2^-31 of the values, 2^-23 of the largest.
+__device__ __forceinline__ bool fixed_fits(uint32_t bits) {
+    return bits == 0 || ((int)(bits >> 23) >= 127 - 8 && (int)(bits >> 23) < 127 + 9);
+}
+__device__ __forceinline__ int part_exponent(uint32_t bits) { return fixed_fits(bits) ? kFixedExp : scale_exponent(bits); }
+// The larger of two magnitudes' bits, of finite values.
+__device__ __forceinline__ uint32_t larger(uint32_t bits, float v) {
+    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+    return b < 0x7f800000u ? max(bits, b) : bits;
+}
+// A value as two f16 parts, packed pairwise: hi = v rounded, lo = the rest rounded.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // Shared-memory descriptor of an N-major operand (rows are K): 64-channel panels of 128-byte rows,
@@ -272,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         }
         for (int i = 0; i < 2; ++i) mbar_init(bar(kSFull + i), 2), mbar_init(bar(kPFull + i), 128);
         for (int i = 0; i < 2; ++i) mbar_init(bar(kOFull + i), 1), mbar_init(bar(kOEmpty + i), 128);
-        mbar_init(bar(kQFull), 1), mbar_init(bar(kFin), 1);
+        mbar_init(bar(kQFull), SPLIT ? 128 : 1), mbar_init(bar(kFin), 1);
         abort_flag = 0, listed = 0;
         fence_mbarrier_init();
     }
@@ -311,25 +330,52 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         // 0, or far below what matters) keeps −inf · c = −inf.
         float c = fabsf(a.scale);
         int ev = 0;
-        if (SPLIT) {
-            const uint32_t* kv = args.amax + args.n * a.heads + (int64_t)item * a.kv_heads + kh;
-            ev = scale_exponent(kv[args.n * a.kv_heads]);
-            c = ldexpf(c, -(scale_exponent(args.amax[(int64_t)item * a.heads + h]) + scale_exponent(*kv)));
+        if constexpr (SPLIT) {
+            // The thread's query row in two parts, at a power of two of its own.
+            const int64_t row = (int64_t)qb * kRows + threadIdx.x;
+            const float* x = static_cast<const float*>(a.q) + ((int64_t)item * a.nq + row) * a.q_stride + (int64_t)h * a.dim;
+            uint32_t top = 0;
+            if (row < a.nq)
+                for (int i = 0; i < a.dim; i += 8) {
+                    float v[8];
+                    widen8<float>(load_raw8(x + i), v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = larger(top, v[e]);
+                }
+            const int eq = scale_exponent(top);
+            const float f = ldexpf(1.0f, eq);
+            uint8_t* to = gbase + (sq - base) + threadIdx.x * 128;
+#pragma unroll 4
+            for (int i = 0; i < (a.dim + 15) / 16 * 16; i += 8) {  // a 16-byte piece, at its swizzled place
+                float v[8] = {};
+                if (row < a.nq && i < a.dim) widen8<float>(load_raw8(x + i), v);
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split2(v[2 * e] * f, v[2 * e + 1] * f, hi[e], lo[e]);
+                const int at = (i >> 6) * (int)kQPanel + (((i >> 3) & 7) ^ (threadIdx.x & 7)) * 16;
+                *reinterpret_cast<uint4*>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(to + at + PANELS * kQPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(bar(kQFull));
+            const uint32_t* kv = args.amax + (int64_t)item * a.kv_heads + kh;
+            ev = part_exponent(kv[args.n * a.kv_heads]);
+            c = ldexpf(c, -(eq + part_exponent(*kv)));
         }
         c = fmaxf(c, 1.17549435e-38f);
         float ref = -INFINITY, l = 0.0f;  // what the weights are relative to, in units of S; their sum
         float acc[SPLIT ? DCOLS : 1];
 #pragma unroll
         for (int i = 0; i < (SPLIT ? DCOLS : 1); ++i) acc[i] = 0.0f;
-        // f32: adds the product of tile t, and brings the sum to the reference that holds since, 2^f lower.
-        auto fold = [&](int t, float f) {
+        // f32: adds the product of tile t to the row's sum.
+        auto fold = [&](int t) {
 #pragma unroll
-            for (int i = 0; i < (SPLIT ? DCOLS : 0); i += 32) {
-                uint32_t o[32];
-                tmem_ld32_wait(lanes + kColO + (t & 1) * DCOLS + i, o);
+            for (int i = 0; i < (SPLIT ? DCOLS : 0); i += 16) {
+                if (i >= a.dim) continue;
+                uint32_t o[16];
+                tmem_ld16_wait(lanes + kColO + (t & 1) * DCOLS + i, o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    acc[SPLIT ? i + e : 0] = (acc[SPLIT ? i + e : 0] + __uint_as_float(o[e])) * f;
+                for (int e = 0; e < 16; ++e) acc[SPLIT ? i + e : 0] += __uint_as_float(o[e]);
             }
         };
         bool ok = true;
@@ -340,21 +386,34 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             if (!ok) break;
             tc_fence_after();
             const uint32_t w0 = valid[slot][0], w1 = valid[slot][1];
-            uint32_t s[kKeys];
-            tmem_ld64_wait(sp, s);
-            if ((w0 & w1) != 0xffffffffu) {
+            // S in registers: all of it, or for f32, whose sums are there too, 32 columns at a time (and again later).
+            constexpr int CH = SPLIT ? 32 : kKeys;
+            uint32_t s[CH];
+            auto read = [&](int q) {
+                if constexpr (SPLIT)
+                    tmem_ld32_wait(sp + q * CH, s);
+                else
+                    tmem_ld64_wait(sp, s);
+                if ((w0 & w1) != 0xffffffffu) {
 #pragma unroll
-                for (int i = 0; i < kKeys; ++i)
-                    if (!((i < 32 ? w0 : w1) >> (i & 31) & 1u)) s[i] = 0xff800000u;
+                    for (int i = 0; i < CH; ++i)
+                        if (!((q * CH + i < 32 ? w0 : w1) >> (i & 31) & 1u)) s[i] = 0xff800000u;
+                }
+            };
+            float top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < kKeys / CH; ++q) {
+                read(q);
+                float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < CH; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(s[i]));
+                top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
             }
-            float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(s[i]));
-            const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-            // Raise the reference: to every new maximum (f32), or when a weight would pass 2^8.
-            const bool raise = SPLIT || ref == -INFINITY ? top > ref : (top - ref) * c > kLazy;
+            // Raise the reference when a weight would pass 2^8.
+            const bool raise = ref == -INFINITY ? top > ref : (top - ref) * c > kLazy;
+            const bool any = __any_sync(0xffffffffu, raise);
             float f = 1.0f;
-            if (__any_sync(0xffffffffu, raise)) {
+            if (any) {
                 if (raise) {
                     f = ref == -INFINITY ? 0.0f : ex2((ref - top) * c);
                     ref = top;
@@ -378,20 +437,22 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             float sum[4] = {};
 #pragma unroll
             for (int q = 0; q < kKeys / 32; ++q) {  // 32 keys: 16 columns of P, and for f32 16 more of its low part
+                if (SPLIT) read(q);
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float p0 = ex2(fmaf(__uint_as_float(s[q * 32 + 2 * i]), c, -mc));
-                    const float p1 = ex2(fmaf(__uint_as_float(s[q * 32 + 2 * i + 1]), c, -mc));
+                    const int at = (SPLIT ? 0 : q * 32) + 2 * i;
+                    const float p0 = ex2(fmaf(__uint_as_float(s[at]), c, -mc));
+                    const float p1 = ex2(fmaf(__uint_as_float(s[at + 1]), c, -mc));
                     sum[i & 1] += p0, sum[2 + (i & 1)] += p1;
-                    hi[i] = pack2(p0, p1, Part());
-                    if (SPLIT) {
-                        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-                        lo[i] = pack2(p0 - b.x, p1 - b.y, Part());
-                    }
+                    if constexpr (SPLIT)
+                        split2(p0, p1, hi[i], lo[i]);
+                    else
+                        hi[i] = pack2(p0, p1, Part());
                 }
-                tmem_st16_u32(pp + q * 16, hi);
-                if (SPLIT) tmem_st16_u32(pp + kKeys / 2 + q * 16, lo);
+                // f32 parts lie over the 32 columns of S that they come from.
+                tmem_st16_u32(pp + q * (SPLIT ? 32 : 16), hi);
+                if (SPLIT) tmem_st16_u32(pp + q * 32 + 16, lo);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_wait_st();
@@ -401,7 +462,11 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                 ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 22);
                 if (!ok) break;
                 tc_fence_after();
-                fold(j - 1, f);
+                fold(j - 1);
+                if (any) {  // brought to the reference that holds from this tile on
+#pragma unroll
+                    for (int i = 0; i < (SPLIT ? DCOLS : 0); ++i) acc[SPLIT ? i : 0] *= f;
+                }
                 tc_fence_before();
                 mbar_arrive(bar(kOEmpty + ((j - 1) & 1)));
             }
@@ -412,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             const int64_t row = (int64_t)qb * kRows + warp * 32 + lane;
             const bool store = row < a.nq;
             const int64_t at = ((int64_t)item * a.nq + row) * a.heads + h;
-            if (SPLIT && tiles > 0) fold(tiles - 1, 1.0f);
+            if (SPLIT && tiles > 0) fold(tiles - 1);
             // One factor for the row: 1 / l, or for a share of the list the weights' own scale taken out.
             const float f = a.splits > 1 ? (SPLIT ? ldexpf(1.0f, -ev - kWeightExp) : 1.0f)
                                          : (l == 0.0f ? 0.0f : (SPLIT ? ldexpf(1.0f, -ev) : 1.0f) / l);
@@ -458,8 +523,8 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             __syncwarp();
         };
         int q_done = 0, k_done = 0, v_done = 0;
-        if (tiles > 0) {
-            load(&map_q, sq, PANELS * PLANES * kQPanel, kQFull, h, qb * kRows, 1, kRows);
+        if (!SPLIT && tiles > 0) {
+            load(&map_q, sq, PANELS * kQPanel, kQFull, h, qb * kRows, 1, kRows);
             q_done = 1;
         }
         // The list and the mask are read ahead of the tiles that they are for: a lane holds the first token of one
@@ -590,11 +655,11 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
 #pragma unroll
                 for (int p = SPLIT ? 0 : 2; p < 3; ++p) {
                     const uint64_t va = v_desc + ((uint32_t)st * OP >> 4) + (p == 1 ? PANELS * kPanel >> 4 : 0);
-                    const uint32_t pa = tmem + PCOL + (j & 1) * PSTEP + (p == 0 ? kKeys / 2 : 0);
+                    const uint32_t pa = tmem + PCOL + (j & 1) * PSTEP;
 #pragma unroll
                     for (int s = 0; s < kKeys / 16; ++s) {
                         const bool fresh = s == 0 && (SPLIT ? p == 0 : j == 0);
-                        mma_16_ts(tmem + kColO + (SPLIT ? (j & 1) * DCOLS : 0), pa + (uint32_t)s * 8u,
+                        mma_16_ts(tmem + kColO + (SPLIT ? (j & 1) * DCOLS : 0), pa + (SPLIT ? (s >> 1) * 32 + (s & 1) * 8 + (p == 0 ? 16 : 0) : s * 8),
                                   va + (uint32_t)(s * 2048 >> 4), idesc_o, fresh ? 0u : 1u);
                     }
                 }
@@ -619,68 +684,74 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
 // ------------------------------------------------------------------------------------ f32 operands
 
 struct SplitArgs {
-    const float *x[3];           // q, k, v
-    int64_t stride[3], rows[3];  // elements between rows; rows of an item
-    int heads[3];
-    __half* parts[3];            // [2][n][rows][heads][dim]
-    uint32_t* amax;
-    int64_t n;
-    int dim;
-    const uint8_t* mask;         // k and v: rows that count
+    const float* x[2];    // k, v
+    int64_t stride[2];    // elements between rows
+    __half* parts[2];     // [2][n][rows][heads][dim]
+    uint32_t* amax;       // [2][n][heads]
+    int64_t n, rows;
+    int heads, dim;
+    const uint8_t* mask;  // rows that count
 };
 
 constexpr int kSplitRows = 64;
+constexpr int kSplitThreads = 256;
 
-// The largest finite magnitude of every (item, head) of q, k and v; the block's y is 3 · (group of 32 chunks) + tensor.
-__global__ void __launch_bounds__(256) attention_amax_kernel(const __grid_constant__ SplitArgs a) {
-    const int t = blockIdx.y % 3, chunk = blockIdx.y / 3 * 32 + (threadIdx.x & 31);
-    const int64_t item = blockIdx.z, r0 = (int64_t)blockIdx.x * kSplitRows;
-    if (r0 >= a.rows[t] || chunk * 8 >= a.heads[t] * a.dim) return;
-    const int64_t r1 = min(r0 + kSplitRows, a.rows[t]);
+// x · 2^e in two parts: 64 rows × 32 pieces of 8 channels. Rows that the mask hides become zero.
+__device__ __forceinline__ uint32_t split_rows(const SplitArgs& a, int t, int64_t item, int64_t r0, int piece, float f) {
+    const int width = a.heads * a.dim;
+    const int64_t plane = a.n * a.rows * width, r1 = min(r0 + kSplitRows, a.rows);
     uint32_t top = 0;
 #pragma unroll 4
-    for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
-        if (t > 0 && a.mask && !a.mask[item * a.rows[t] + r]) continue;
-        float v[8];
-        widen8<float>(load_raw8(a.x[t] + (item * a.rows[t] + r) * a.stride[t] + chunk * 8), v);
+    for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += kSplitThreads / 32) {
+        const int64_t row = item * a.rows + r;
+        float v[8] = {};
+        if (!a.mask || a.mask[row]) widen8<float>(load_raw8(a.x[t] + row * a.stride[t] + piece * 8), v);
+        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-            if (b < 0x7f800000u) top = max(top, b);
+        for (int e = 0; e < 4; ++e) {
+            top = larger(larger(top, v[2 * e]), v[2 * e + 1]);
+            split2(v[2 * e] * f, v[2 * e + 1] * f, hi[e], lo[e]);
         }
+        uint4* out = reinterpret_cast<uint4*>(a.parts[t] + row * width + piece * 8);
+        out[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        out[plane / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    const int64_t first = t == 0 ? 0 : a.n * (a.heads[0] + (t - 1) * a.heads[1]);
-    if (top) atomicMax(a.amax + first + item * a.heads[t] + chunk * 8 / a.dim, top);
+    return top;
 }
 
-// x · 2^e as two f16 parts; rows that the mask hides become zero.
-__global__ void __launch_bounds__(256) attention_split_kernel(const __grid_constant__ SplitArgs a) {
-    const int t = blockIdx.y % 3, chunk = blockIdx.y / 3 * 32 + (threadIdx.x & 31);
-    const int64_t item = blockIdx.z, r0 = (int64_t)blockIdx.x * kSplitRows;
-    const int width = a.heads[t] * a.dim;
-    if (r0 >= a.rows[t] || chunk * 8 >= width) return;
-    const int64_t first = t == 0 ? 0 : a.n * (a.heads[0] + (t - 1) * a.heads[1]);
-    const int e = scale_exponent(a.amax[first + item * a.heads[t] + chunk * 8 / a.dim]);
-    const float f = ldexpf(1.0f, e);
-    const int64_t r1 = min(r0 + kSplitRows, a.rows[t]), plane = a.n * a.rows[t] * width;
-#pragma unroll 4
-    for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
-        const int64_t row = item * a.rows[t] + r;
-        float v[8], lo[8];
-        if (t > 0 && a.mask && !a.mask[row]) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        } else {
-            widen8<float>(load_raw8(a.x[t] + row * a.stride[t] + chunk * 8), v);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[i] *= f;
-            lo[i] = v[i] - __half2float(__float2half_rn(v[i]));
-        }
-        __half* out = a.parts[t] + row * width + chunk * 8;
-        store8(out, v);
-        store8(out + plane, lo);
+// One pass over k and v: their parts at the exponent that fits almost any head, and what tells whether it does, the
+// largest finite magnitude of each head. A pass for the magnitudes alone would read everything twice: 126 us
+// for 252 MB beside 97 us for the parts.
+__global__ void __launch_bounds__(kSplitThreads) attention_split_kernel(const __grid_constant__ SplitArgs a) {
+    __shared__ uint32_t tops[32];
+    const int t = blockIdx.y & 1, lane = threadIdx.x & 31, piece = (blockIdx.y >> 1) * 32 + lane;
+    const int64_t item = blockIdx.z;
+    if (threadIdx.x < 32) tops[threadIdx.x] = 0;
+    __syncthreads();
+    const bool on = piece * 8 < a.heads * a.dim;
+    uint32_t top = 0;
+    if (on) top = split_rows(a, t, item, (int64_t)blockIdx.x * kSplitRows, piece, ldexpf(1.0f, kFixedExp));
+    const int first = (blockIdx.y >> 1) * 256 / a.dim, head = piece * 8 / a.dim;  // at most 32 heads: dim >= 8
+    if (on) atomicMax(&tops[head - first], top);
+    __syncthreads();
+    if (threadIdx.x < 32 && tops[threadIdx.x])
+        atomicMax(a.amax + (t * a.n + item) * a.heads + first + threadIdx.x, tops[threadIdx.x]);
+}
+
+// The heads that the fixed exponent does not fit, once more with their own.
+__global__ void __launch_bounds__(kSplitThreads) attention_resplit_kernel(const __grid_constant__ SplitArgs a) {
+    const int64_t total = 2 * a.n * a.heads;
+    bool none = true;
+    for (int64_t i = threadIdx.x; i < total; i += kSplitThreads) none &= fixed_fits(a.amax[i]);
+    if (__syncthreads_and(none)) return;
+    const int groups = (a.heads * a.dim / 8 + 31) / 32;
+    const int64_t tiles = (a.rows + kSplitRows - 1) / kSplitRows, all = tiles * groups * 2 * a.n;
+    for (int64_t w = blockIdx.x; w < all; w += gridDim.x) {
+        const int t = (int)(w & 1), piece = (int)(w / 2 % groups) * 32 + (threadIdx.x & 31);
+        const int64_t item = w / 2 / groups / tiles, tile = w / 2 / groups % tiles;
+        if (piece * 8 >= a.heads * a.dim) continue;
+        const uint32_t bits = a.amax[(t * a.n + item) * a.heads + piece * 8 / a.dim];
+        if (!fixed_fits(bits)) split_rows(a, t, item, tile * kSplitRows, piece, ldexpf(1.0f, scale_exponent(bits)));
     }
 }
 
@@ -706,43 +777,42 @@ void launch_typed(mbx_ctx* ctx, const TcArgs& t, const CUtensorMap (&maps)[3]) {
 }  // namespace
 
 size_t attention_split_bytes(const BlockShape& s) {
-    return align256(4 * (size_t)(s.n * (s.heads + 2 * s.kv_heads))) + 2 * 2 * (size_t)(s.n * s.nq * s.heads * s.dim) +
-           2 * 2 * 2 * (size_t)(s.n * s.nk * s.kv_heads * s.dim) + 256;
+    return align256(4 * 2 * (size_t)(s.n * s.kv_heads)) +
+           2 * align256(2 * 2 * (size_t)(s.n * s.nk * s.kv_heads * s.dim));
 }
 
 void launch_attention_tc(mbx_ctx* ctx, const AttnArgs& a, int dtype, int64_t n, void* split) {
     TcArgs t{a, nullptr, n, ctx->dev_err};
-    const void* x[3] = {a.q, a.k, a.v};
-    int64_t stride[3] = {a.q_stride, a.k_stride, a.v_stride};
-    const int64_t rows[3] = {a.nq, a.nk, a.nk}, heads[3] = {a.heads, a.kv_heads, a.kv_heads};
-    int planes = 1;
-    if (dtype == MBX_DTYPE_F32) {
-        planes = 2;
-        SplitArgs s{};
-        s.amax = static_cast<uint32_t*>(split);
-        const size_t amax_bytes = 4 * (size_t)(n * (a.heads + 2 * a.kv_heads));
-        uint8_t* at = static_cast<uint8_t*>(split) + align256(amax_bytes);
-        for (int i = 0; i < 3; ++i) {
-            s.x[i] = static_cast<const float*>(x[i]), s.stride[i] = stride[i], s.rows[i] = rows[i];
-            s.heads[i] = (int)heads[i];
-            s.parts[i] = reinterpret_cast<__half*>(at);
-            at += 2 * 2 * (size_t)(n * rows[i] * heads[i] * a.dim);
-            x[i] = s.parts[i], stride[i] = heads[i] * a.dim;
-        }
-        s.n = n, s.dim = a.dim, s.mask = a.mask;
-        check_cuda(cudaMemsetAsync(s.amax, 0, amax_bytes, ctx->stream), "cudaMemsetAsync");
-        const dim3 grid((unsigned)((std::max(a.nq, a.nk) + kSplitRows - 1) / kSplitRows),
-                        (unsigned)(3 * ((a.heads * a.dim / 8 + 31) / 32)), (unsigned)n);
-        attention_amax_kernel<<<grid, 256, 0, ctx->stream>>>(s);
-        after_launch(ctx, "attention_amax");
-        attention_split_kernel<<<grid, 256, 0, ctx->stream>>>(s);
-        after_launch(ctx, "attention_split");
-        t.amax = s.amax;
-    }
     CUtensorMap maps[3];
-    for (int i = 0; i < 3; ++i)
-        encode_heads(&maps[i], x[i], dtype == MBX_DTYPE_BF16, planes * n, rows[i], heads[i], a.dim, stride[i],
-                     i == 0 ? kRows : std::min(a.block_k, kKeys));
+    const bool bf16 = dtype == MBX_DTYPE_BF16;
+    const int rows_box = std::min(a.block_k, kKeys);
+    if (dtype == MBX_DTYPE_F32) {
+        SplitArgs s{};
+        const size_t amax_bytes = 4 * 2 * (size_t)(n * a.kv_heads);
+        const size_t part_bytes = align256(2 * 2 * (size_t)(n * a.nk * a.kv_heads * a.dim));
+        s.amax = static_cast<uint32_t*>(split);
+        s.n = n, s.rows = a.nk, s.heads = a.kv_heads, s.dim = a.dim, s.mask = a.mask;
+        s.x[0] = static_cast<const float*>(a.k), s.x[1] = static_cast<const float*>(a.v);
+        s.stride[0] = a.k_stride, s.stride[1] = a.v_stride;
+        for (int i = 0; i < 2; ++i)
+            s.parts[i] = reinterpret_cast<__half*>(static_cast<uint8_t*>(split) + align256(amax_bytes) + i * part_bytes);
+        check_cuda(cudaMemsetAsync(s.amax, 0, amax_bytes, ctx->stream), "cudaMemsetAsync");
+        const dim3 grid((unsigned)((a.nk + kSplitRows - 1) / kSplitRows),
+                        (unsigned)(2 * ((a.kv_heads * a.dim / 8 + 31) / 32)), (unsigned)n);
+        attention_split_kernel<<<grid, kSplitThreads, 0, ctx->stream>>>(s);
+        after_launch(ctx, "attention_split");
+        attention_resplit_kernel<<<ctx->sm_count, kSplitThreads, 0, ctx->stream>>>(s);
+        after_launch(ctx, "attention_resplit");
+        t.amax = s.amax;
+        for (int i = 1; i < 3; ++i)
+            encode_heads(&maps[i], s.parts[i - 1], false, 2 * n, a.nk, a.kv_heads, a.dim, (int64_t)a.kv_heads * a.dim,
+                         rows_box);
+        maps[0] = maps[1];  // q is split where it is used
+    } else {
+        encode_heads(&maps[0], a.q, bf16, n, a.nq, a.heads, a.dim, a.q_stride, kRows);
+        encode_heads(&maps[1], a.k, bf16, n, a.nk, a.kv_heads, a.dim, a.k_stride, rows_box);
+        encode_heads(&maps[2], a.v, bf16, n, a.nk, a.kv_heads, a.dim, a.v_stride, rows_box);
+    }
     if (dtype == MBX_DTYPE_F32) return a.dim > 64 ? launch_typed<float, 2>(ctx, t, maps) : launch_typed<float, 1>(ctx, t, maps);
     if (dtype == MBX_DTYPE_F16) return a.dim > 64 ? launch_typed<__half, 2>(ctx, t, maps) : launch_typed<__half, 1>(ctx, t, maps);
     a.dim > 64 ? launch_typed<__nv_bfloat16, 2>(ctx, t, maps) : launch_typed<__nv_bfloat16, 1>(ctx, t, maps);
