@@ -116,30 +116,60 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const At
         if (a.splits == 1) {
             static_cast<T*>(a.out)[row * a.dim + ch] = (T)(sum == 0.0f ? 0.0f : o / sum);
         } else {
-            float* p = a.part + (row * a.splits + split) * (a.dim + 2);
+            float* p = a.part + (row * a.splits + split) * (a.dim + 4);
             p[ch] = o;
             if (ch == 0) p[a.dim] = top, p[a.dim + 1] = sum;
         }
     }
 }
 
-// Joins the splits' partial results: one warp per (row, head).
+// Joins the splits' partial results: a CTA per (row, head). The splits' weights are worked out once in shared memory;
+// then each warp adds every fourth split, a lane four channels, eight splits in flight.
+constexpr int kMaxSplits = 64;
+
 template <class T>
-__global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a, int64_t rows) {
-    const int64_t row = blockIdx.x * 4ll + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const float* p = a.part + row * a.splits * (a.dim + 2);
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, p[s * (a.dim + 2) + a.dim]);
-    for (int ch = threadIdx.x & 31; ch < a.dim; ch += 32) {
-        float sum = 0.0f, o = 0.0f;
-        for (int s = 0; s < a.splits; ++s) {
-            const float* ps = p + s * (a.dim + 2);
-            const float w = ps[a.dim] == -INFINITY ? 0.0f : exp2f(ps[a.dim] - top);
-            sum = fmaf(w, ps[a.dim + 1], sum);
-            o = fmaf(w, ps[ch], o);
+__global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a) {
+    __shared__ float weight[kMaxSplits];
+    __shared__ float4 acc[4][32];
+    __shared__ float total;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stride = a.dim + 4;
+    const float* p = a.part + (int64_t)blockIdx.x * a.splits * stride;
+    if (warp == 0) {
+        float m[2], l[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int s = lane + 32 * i;
+            m[i] = s < a.splits ? p[s * stride + a.dim] : -INFINITY;
+            l[i] = s < a.splits ? p[s * stride + a.dim + 1] : 0.0f;
         }
-        static_cast<T*>(a.out)[row * a.dim + ch] = (T)(sum == 0.0f ? 0.0f : o / sum);
+        float top = fmaxf(m[0], m[1]);
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float w = m[i] == -INFINITY ? 0.0f : exp2f(m[i] - top);
+            weight[lane + 32 * i] = w;
+            sum = fmaf(w, l[i], sum);
+        }
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) total = sum;
+    }
+    __syncthreads();
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (lane * 4 < a.dim) {
+#pragma unroll 8
+        for (int s = warp; s < a.splits; s += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + s * stride + lane * 4);
+            const float w = weight[s];
+            o = f4_fma(make_float4(w, w, w, w), v, o);
+        }
+    }
+    acc[warp][lane] = o;
+    __syncthreads();
+    if ((int)threadIdx.x < a.dim) {
+        const float* x = reinterpret_cast<const float*>(acc);
+        const float y = (x[threadIdx.x] + x[128 + threadIdx.x]) + (x[256 + threadIdx.x] + x[384 + threadIdx.x]);
+        static_cast<T*>(a.out)[(int64_t)blockIdx.x * a.dim + threadIdx.x] = (T)(total == 0.0f ? 0.0f : y / total);
     }
 }
 
@@ -160,9 +190,9 @@ Plan plan_of(const BlockShape& s, int64_t topk) {
     const int64_t tile = p.rows ? kRowsR : MBX_ATTENTION_BLOCK_Q;
     const int64_t ctas = std::max<int64_t>(1, s.n * s.heads * ((s.nq + tile - 1) / tile));
     const int64_t pieces = p.rows ? topk : (topk * s.block_k + 63) / 64;
-    p.splits = (int)std::max<int64_t>(1, std::min({(2 * kSms + ctas - 1) / ctas, pieces, int64_t(64)}));
+    p.splits = (int)std::max<int64_t>(1, std::min({(2 * kSms + ctas - 1) / ctas, pieces, int64_t(kMaxSplits)}));
     if (p.splits > 1)
-        p.part_bytes = align256(sizeof(float) * (size_t)(s.n * s.nq * s.heads) * p.splits * (s.dim + 2));
+        p.part_bytes = align256(sizeof(float) * (size_t)(s.n * s.nq * s.heads) * p.splits * (s.dim + 4));
     if (!p.rows && s.dtype == MBX_DTYPE_F32) p.split_bytes = attention_split_bytes(s);
     return p;
 }
@@ -183,7 +213,8 @@ void launch_rows(mbx_ctx* ctx, const AttnArgs& a, int64_t n) {
 template <class T>
 void launch_join(mbx_ctx* ctx, const AttnArgs& a, int64_t n) {
     const int64_t rows = n * a.nq * a.heads;
-    attention_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, ctx->stream>>>(a, rows);
+    MBX_REQUIRE(rows < (int64_t(1) << 31), "block_attention: too many query rows");
+    attention_join_kernel<T><<<(unsigned)rows, 128, 0, ctx->stream>>>(a);
     after_launch(ctx, "attention_join");
 }
 

@@ -2,18 +2,24 @@
 // TMA-fed operands).
 //
 // A CTA takes one query block (128 rows) of one (item, head), or a share of its list, and walks
-// the listed key blocks in tiles of 64 keys (a part of a block, or several blocks with a TMA box
-// each, so any block size feeds the same tile). Six warps:
+// the listed key blocks in tiles of 64 or 128 keys (a part of a block, or several blocks with a TMA
+// box each, so any block size feeds the same tile). Seven warps:
 //   warps 0-3  softmax: a thread owns a query row (a TMEM lane). It reads S from TMEM, keeps the
 //              running maximum and sum in f32 registers and writes the weights 2^(c·s − c·m)
 //              back to TMEM, as the second product's left operand.
-//   warp 4     producer: TMA for Q once and for K, V of every tile; the tile's bits of valid keys.
-//   warp 5     MMA issuer (one thread) and TMEM allocation.
-// TMEM: two S tiles of 64 columns, two P tiles (16-bit, up to 64 channels; else P lies over its S)
-// and O. While the weights of one tile are computed, Q·Kᵀ of the next runs into the other, so the softmax warps work back to back,
-// and two CTAs share an SM (one for f32 with more than 64 channels). 64 keys and not 128: two S
-// tiles of 128 columns and O would leave one CTA an SM; the price is Q·Kᵀ at N = 64, where reading
-// Q from shared memory takes 1.5 times the product's own cycles.
+//   warps 4, 6 producers: TMA for Q once and for K of every tile, with the tile's bits of valid keys; TMA
+//              for V. (One warp for both would hold back the next K until P·V frees a V stage.)
+//   warp 5     MMA issuer (one lane) and TMEM allocation.
+// Two CTAs share an SM (one for f32 with more than 64 channels), 256 TMEM columns each, and two ways
+// to let a tile's Q·Kᵀ run while the softmax warps work on the tile before it:
+//   16-bit, up to 64 channels: tiles of 128 keys, S, a P of its own and O (128 + 64 + 64 columns). Q·Kᵀ
+//     of the next tile begins when S has been read for the last time, half way through the weights.
+//   otherwise: tiles of 64 keys, two S tiles in turn, P over its S, and O (f32: twice). Q·Kᵀ of the tile
+//     after the next begins when P·V has read P. The price is N = 64, at which reading Q from shared
+//     memory takes 1.5 times the product's own cycles; with one S tile of 128 keys instead, P·V and Q·Kᵀ
+//     stand between two softmax steps (1.3 times the time at 128 channels).
+// A tile's fixed costs in the softmax warps (waits, exchange, addresses: some 400 of 1570 cycles for 64 keys)
+// are what the longer tile halves. Two threads a row, for twice the warps, cost more than they hid.
 // Shared memory: Q, K and V in 128-byte-swizzled panels of 64 channels; V serves as the N-major
 // operand as it lies, so nothing is transposed.
 //
@@ -25,10 +31,9 @@
 // f32 operands: two f16 parts of every value after a power-of-two scale (k and v beforehand, by
 // head; a query row by the thread that owns it, as it begins): a value is held to 2^-23 of itself or of
 // the largest. Three products (lo·hi, hi·lo, hi·hi; lo·lo is 2^-22 of the whole), and the weights in
-// two parts after a scale of 2^7. The tensor core truncates as it adds into its f32
-// accumulator, so a long sum there drifts by about 2^-25 a step: each tile's P·V starts a fresh
-// accumulator (two in turn) and the softmax threads add it to f32 registers, rounding to nearest,
-// after they have handed over the next tile's weights.
+// two parts after a scale of 2^7. The tensor core truncates as it adds into its f32 accumulator, so a
+// long sum there drifts by about 2^-25 a step: after every 4 tiles the softmax threads add what has been
+// gathered to a second set of TMEM columns, rounding to nearest, and the next tile begins a fresh sum.
 //
 // Masked keys: S becomes −inf; their V rows become zero in shared memory (16-bit) or while
 // splitting (f32), since zero times what a mask hides may be NaN.
@@ -45,12 +50,11 @@ namespace mbx {
 namespace {
 
 constexpr int kRows = MBX_ATTENTION_BLOCK_Q;
-constexpr int kKeys = 64;                   // keys of a tile
 constexpr uint32_t kQPanel = kRows * 128;   // bytes of 64 channels of the query block
-constexpr uint32_t kPanel = kKeys * 128;    // and of a tile of K or V
-constexpr int kThreads = 192;
-// Tiles whose bits of valid keys are kept: a slot is written again 8 tiles on, when Q·Kᵀ of 8 − stages tiles on is
-// complete, which was begun after P·V of two tiles before it, and so after this tile's bits were read (stages <= 6).
+constexpr int kThreads = 224;
+constexpr int kSegment = 4;                 // f32: tiles of one unbroken sum (256 keys)
+// Tiles whose bits of valid keys are kept: a slot is written again 8 tiles on, when Q·Kᵀ of a tile at most 4 before
+// that is complete, which was begun when the tile two before it, or a later one, had been read.
 constexpr int kMaskSlots = 8;
 constexpr float kLazy = 8.0f;   // log2 of the largest weight
 constexpr int kWeightExp = 7;   // f32 operands: weights are scaled by 2^7 before their split, up to 2^15
@@ -64,28 +68,28 @@ struct TcArgs {
     int* err;
 };
 
-template <int PANELS, bool SPLIT>
-constexpr int stages_of() {
-    return !SPLIT && PANELS == 1 ? 4 : 2;
-}
-
-// TMEM: two S tiles; two P tiles of their own where that still leaves two CTAs an SM; O, two of them for f32.
+// The two layouts (above).
 template <int PANELS, bool SPLIT>
 constexpr bool own_p() {
     return PANELS == 1 && !SPLIT;
 }
 template <int PANELS, bool SPLIT>
+constexpr int keys_of() {
+    return own_p<PANELS, SPLIT>() ? 128 : 64;
+}
+template <int PANELS, bool SPLIT>
 constexpr uint32_t col_o() {
-    return 2 * kKeys + (own_p<PANELS, SPLIT>() ? kKeys : 0);
+    return own_p<PANELS, SPLIT>() ? 128 + 64 : 2 * 64;
 }
 template <int PANELS, bool SPLIT>
 constexpr uint32_t tmem_cols() {
     return col_o<PANELS, SPLIT>() + PANELS * 64 * (SPLIT ? 2 : 1) <= 256 ? 256 : 512;
 }
+constexpr int kStages = 2;  // tiles of K, and of V, in shared memory
 
 template <int PANELS, bool SPLIT>
 constexpr int smem_of() {
-    return PANELS * (SPLIT ? 2 : 1) * (int)(kQPanel + 2 * stages_of<PANELS, SPLIT>() * kPanel) + 1024;
+    return PANELS * (SPLIT ? 2 : 1) * (int)(kQPanel + 2 * kStages * keys_of<PANELS, SPLIT>() * 128) + 1024;
 }
 
 // Columns of the warp's 32 lanes, complete on return: the wait is part of the statement, so that nothing that uses the
@@ -98,20 +102,6 @@ __device__ __forceinline__ void tmem_ld16_wait(uint32_t taddr, uint32_t (&r)[16]
         "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld32_wait(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
-        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31 "
-        "}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr)
         : "memory");
 }
@@ -150,6 +140,12 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return y;
+}
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -184,11 +180,11 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 }
 
 // Shared-memory descriptor of an N-major operand (rows are K): 64-channel panels of 128-byte rows,
-// 128-byte swizzle; 8-row groups 1024 bytes apart (SBO), panels kPanel apart (LBO).
-__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr) {
+// 128-byte swizzle; 8-row groups 1024 bytes apart (SBO), panels `panel` bytes apart (LBO).
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t panel) {
     uint64_t d = 0;
     d |= (uint64_t)((saddr & 0x3ffffu) >> 4);
-    d |= (uint64_t)(kPanel >> 4) << 16;
+    d |= (uint64_t)(panel >> 4) << 16;
     d |= (uint64_t)(1024 >> 4) << 32;
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
@@ -237,17 +233,19 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
     constexpr bool SPLIT = is_f32<OUT>();
     constexpr bool BF16 = std::is_same<OUT, __nv_bfloat16>::value;
     constexpr int PLANES = SPLIT ? 2 : 1;
-    constexpr int STAGES = stages_of<PANELS, SPLIT>();
+    constexpr int STAGES = kStages, KEYS = keys_of<PANELS, SPLIT>(), WORDS = KEYS / 32;
+    constexpr uint32_t kPanel = KEYS * 128;            // bytes of 64 channels of a tile of K or V
     constexpr uint32_t OP = PANELS * PLANES * kPanel;  // bytes of a tile of K or V
     constexpr uint32_t TMEM = tmem_cols<PANELS, SPLIT>(), kColO = col_o<PANELS, SPLIT>();
     constexpr bool OWN_P = own_p<PANELS, SPLIT>();
-    constexpr uint32_t PCOL = OWN_P ? 2 * kKeys : 0, PSTEP = OWN_P ? kKeys / 2 : kKeys;  // P tiles, else over S
+    constexpr int NS = OWN_P ? 1 : 2;  // S tiles
+    constexpr uint32_t PCOL = OWN_P ? KEYS : 0;
     constexpr int DCOLS = PANELS * 64;
     using Part = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     const AttnArgs& a = args.a;
 
-    // Barriers that a tile in two uses come in pairs, one for the even tiles and one for the odd: a
-    // waiter is then never two phases behind, which a parity could not tell from none.
+    // Barriers of S and P, one for each S tile, and of O, one for even and one for odd tiles: a waiter is then never two
+    // phases behind, which a parity could not tell from none.
     enum {
         kKFull = 0,
         kKEmpty = kKFull + STAGES,
@@ -255,18 +253,19 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         kVEmpty = kVFull + STAGES,
         kVClean = kVEmpty + STAGES,
         kQFull = kVClean + STAGES,
-        kSFull,               // [2] a tile's S is complete
-        kPFull = kSFull + 2,  // [2] a tile's weights are written
-        kOFull = kPFull + 2,   // [2] a tile's P·V is complete
-        kOEmpty = kOFull + 2,  // [2] f32: a tile's product is added to the registers
-        kFin = kOEmpty + 2,
+        kSFull,                 // [NS] a tile's S is complete
+        kSEmpty = kSFull + NS,  // and read, where P has columns of its own
+        kPFull,                 // [NS] a tile's weights are written
+        kOFull = kPFull + NS,   // [2] a tile's P·V is complete
+        kOEmpty = kOFull + 2,  // f32: a segment's sum is taken
+        kFin,
         kBars
     };
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[kBars];
-    __shared__ volatile uint32_t valid[kMaskSlots][2];
+    __shared__ volatile uint32_t valid[kMaskSlots][4];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag, listed;
+    __shared__ int abort_flag;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t sv = base, sk = sv + STAGES * OP, sq = sk + STAGES * OP;
@@ -284,35 +283,34 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
     const uint8_t* mask = a.mask ? a.mask + (int64_t)item * a.nk : nullptr;
     const bool cleans = !SPLIT && mask != nullptr;
 
+    // Entries up to the last one that names a block: every warp looks for itself, while the rest is set up.
+    int listed = 0;
+#pragma unroll 2
+    for (int e = lane; e < (int)a.topk; e += 32)
+        if ((uint32_t)list[e] < (uint32_t)a.k_blocks) listed = e + 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(bar(kKFull + i), 1), mbar_init(bar(kKEmpty + i), 1);
             mbar_init(bar(kVFull + i), 1), mbar_init(bar(kVEmpty + i), 1), mbar_init(bar(kVClean + i), 1);
         }
-        for (int i = 0; i < 2; ++i) mbar_init(bar(kSFull + i), 2), mbar_init(bar(kPFull + i), 128);
-        for (int i = 0; i < 2; ++i) mbar_init(bar(kOFull + i), 1), mbar_init(bar(kOEmpty + i), 128);
-        mbar_init(bar(kQFull), SPLIT ? 128 : 1), mbar_init(bar(kFin), 1);
-        abort_flag = 0, listed = 0;
+        for (int i = 0; i < NS; ++i) mbar_init(bar(kSFull + i), 2), mbar_init(bar(kPFull + i), 4);
+        for (int i = 0; i < 2; ++i) mbar_init(bar(kOFull + i), 1);
+        mbar_init(bar(kSEmpty), 4);
+        mbar_init(bar(kQFull), SPLIT ? 4 : 1), mbar_init(bar(kOEmpty), 4), mbar_init(bar(kFin), 1);
+        abort_flag = 0;
         fence_mbarrier_init();
     }
     if (warp == 5) {
         tmem_alloc(smem_u32(&tmem_slot), TMEM);
         tmem_relinquish();
     }
-    __syncthreads();
-    {  // entries up to the last one that names a block
-        int last = 0;
-        for (int e = threadIdx.x; e < (int)a.topk; e += kThreads)
-            if ((uint32_t)list[e] < (uint32_t)a.k_blocks) last = e + 1;
-        last = __reduce_max_sync(0xffffffffu, last);
-        if (lane == 0 && last > 0) atomicMax(&listed, last);
-    }
+    listed = __reduce_max_sync(0xffffffffu, listed);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const int rows_box = min(a.block_k, kKeys), boxes = kKeys / rows_box;  // TMA boxes of a tile
-    const int all_tiles = (int)(((int64_t)listed * a.block_k + kKeys - 1) / kKeys);
+    const int rows_box = min(a.block_k, KEYS), boxes = KEYS / rows_box;  // TMA boxes of a tile
+    const int all_tiles = (int)(((int64_t)listed * a.block_k + KEYS - 1) / KEYS);
     const int t0 = (int)((int64_t)all_tiles * split / a.splits);
     const int tiles = (int)((int64_t)all_tiles * (split + 1) / a.splits) - t0;
     volatile int* abort_p = &abort_flag;
@@ -326,22 +324,29 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
     if (warp < 4) {
         // ---------------------------------------------------------------- softmax
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        const int64_t row = (int64_t)qb * kRows + threadIdx.x;
+        // One arrival for the warp, after everything that its lanes have done.
+        auto arrive = [&](int b) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(b));
+        };
         // A negative scale negates Q in the instruction descriptor. The least normal value in place of 0 (a scale of
         // 0, or far below what matters) keeps −inf · c = −inf.
         float c = fabsf(a.scale);
         int ev = 0;
         if constexpr (SPLIT) {
             // The thread's query row in two parts, at a power of two of its own.
-            const int64_t row = (int64_t)qb * kRows + threadIdx.x;
             const float* x = static_cast<const float*>(a.q) + ((int64_t)item * a.nq + row) * a.q_stride + (int64_t)h * a.dim;
             uint32_t top = 0;
-            if (row < a.nq)
+            if (row < a.nq) {
+#pragma unroll 4
                 for (int i = 0; i < a.dim; i += 8) {
                     float v[8];
                     widen8<float>(load_raw8(x + i), v);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) top = larger(top, v[e]);
                 }
+            }
             const int eq = scale_exponent(top);
             const float f = ldexpf(1.0f, eq);
             uint8_t* to = gbase + (sq - base) + threadIdx.x * 128;
@@ -357,158 +362,162 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                 *reinterpret_cast<uint4*>(to + at + PANELS * kQPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
             fence_proxy_async_smem();
-            mbar_arrive(bar(kQFull));
+            arrive(kQFull);
             const uint32_t* kv = args.amax + (int64_t)item * a.kv_heads + kh;
             ev = part_exponent(kv[args.n * a.kv_heads]);
             c = ldexpf(c, -(eq + part_exponent(*kv)));
         }
         c = fmaxf(c, 1.17549435e-38f);
         float ref = -INFINITY, l = 0.0f;  // what the weights are relative to, in units of S; their sum
-        float acc[SPLIT ? DCOLS : 1];
+        // O's columns, 16 at a time, as far as there are channels.
+        auto columns = [&](auto&& f) {
 #pragma unroll
-        for (int i = 0; i < (SPLIT ? DCOLS : 1); ++i) acc[i] = 0.0f;
-        // f32: adds the product of tile t to the row's sum.
-        auto fold = [&](int t) {
-#pragma unroll
-            for (int i = 0; i < (SPLIT ? DCOLS : 0); i += 16) {
-                if (i >= a.dim) continue;
-                uint32_t o[16];
-                tmem_ld16_wait(lanes + kColO + (t & 1) * DCOLS + i, o);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[SPLIT ? i + e : 0] += __uint_as_float(o[e]);
-            }
+            for (int i = 0; i < DCOLS; i += 16)
+                if (i < a.dim) f(i);
         };
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
             const int slot = j % kMaskSlots;
-            const uint32_t sp = lanes + (j & 1) * kKeys, pp = lanes + PCOL + (j & 1) * PSTEP;  // its S and P
-            ok = warp_wait(kSFull + (j & 1), j >> 1, 21);
+            const int b = j % NS;
+            const uint32_t sp = lanes + b * KEYS, pp = lanes + PCOL + b * KEYS;  // its S and P
+            ok = warp_wait(kSFull + b, j / NS, 21);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t w0 = valid[slot][0], w1 = valid[slot][1];
-            // S in registers: all of it, or for f32, whose sums are there too, 32 columns at a time (and again later).
-            constexpr int CH = SPLIT ? 32 : kKeys;
-            uint32_t s[CH];
-            auto read = [&](int q) {
-                if constexpr (SPLIT)
-                    tmem_ld32_wait(sp + q * CH, s);
-                else
-                    tmem_ld64_wait(sp, s);
-                if ((w0 & w1) != 0xffffffffu) {
+            uint32_t w[WORDS], some = 0xffffffffu;
 #pragma unroll
-                    for (int i = 0; i < CH; ++i)
-                        if (!((q * CH + i < 32 ? w0 : w1) >> (i & 31) & 1u)) s[i] = 0xff800000u;
+            for (int i = 0; i < WORDS; ++i) w[i] = valid[slot][i], some &= w[i];
+            uint32_t s[64];
+            auto read = [&](int q) {  // 64 columns of S
+                tmem_ld64_wait(sp + q * 64, s);
+                if (some != 0xffffffffu) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        if (!(w[q * 2 + (i >> 5)] >> (i & 31) & 1u)) s[i] = 0xff800000u;
                 }
             };
-            float top = -INFINITY;
+            float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int q = 0; q < kKeys / CH; ++q) {
+            for (int q = 0; q < KEYS / 64; ++q) {
                 read(q);
-                float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < CH; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(s[i]));
-                top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+                for (int i = 0; i < 64; i += 2) t[i >> 1 & 3] = max3(t[i >> 1 & 3], s[i], s[i + 1]);
             }
+            const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
             // Raise the reference when a weight would pass 2^8.
             const bool raise = ref == -INFINITY ? top > ref : (top - ref) * c > kLazy;
-            const bool any = __any_sync(0xffffffffu, raise);
-            float f = 1.0f;
-            if (any) {
+            if (__any_sync(0xffffffffu, raise)) {
+                float f = 1.0f;
                 if (raise) {
                     f = ref == -INFINITY ? 0.0f : ex2((ref - top) * c);
                     ref = top;
                 }
                 l *= f;
-                if (!SPLIT && j > 0) {
+                if (j > 0) {
                     ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 22);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < DCOLS; i += 16) {
-                        uint32_t o[16];
-                        tmem_ld16_wait(lanes + kColO + i, o);
+                    for (int r = 0; r < (SPLIT ? 2 : 1); ++r) {
+                        if (r == 1 && j <= kSegment) continue;  // nothing has been taken yet
+                        columns([&](int i) {
+                            uint32_t o[16];
+                            tmem_ld16_wait(lanes + kColO + r * DCOLS + i, o);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st16_u32(lanes + kColO + i, o);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16_u32(lanes + kColO + r * DCOLS + i, o);
+                        });
                     }
                 }
+            }
+            if (OWN_P && j > 0) {  // P of the last tile has been read
+                ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 23);
+                if (!ok) break;
             }
             const float mc = (ref == -INFINITY ? 0.0f : ref) * c - (SPLIT ? (float)kWeightExp : 0.0f);
             float sum[4] = {};
 #pragma unroll
-            for (int q = 0; q < kKeys / 32; ++q) {  // 32 keys: 16 columns of P, and for f32 16 more of its low part
-                if (SPLIT) read(q);
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at = (SPLIT ? 0 : q * 32) + 2 * i;
-                    const float p0 = ex2(fmaf(__uint_as_float(s[at]), c, -mc));
-                    const float p1 = ex2(fmaf(__uint_as_float(s[at + 1]), c, -mc));
-                    sum[i & 1] += p0, sum[2 + (i & 1)] += p1;
-                    if constexpr (SPLIT)
-                        split2(p0, p1, hi[i], lo[i]);
-                    else
-                        hi[i] = pack2(p0, p1, Part());
+            for (int q = KEYS / 64 - 1; q >= 0; --q) {  // the last 64 keys first: they are in registers
+                if (q < KEYS / 64 - 1) {
+                    read(q);
+                    tc_fence_before();
+                    arrive(kSEmpty);
                 }
-                // f32 parts lie over the 32 columns of S that they come from.
-                tmem_st16_u32(pp + q * (SPLIT ? 32 : 16), hi);
-                if (SPLIT) tmem_st16_u32(pp + q * 32 + 16, lo);
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {  // 32 keys: 16 columns of P, and for f32 16 more of its low part
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float p0 = ex2(fmaf(__uint_as_float(s[g * 32 + 2 * i]), c, -mc));
+                        const float p1 = ex2(fmaf(__uint_as_float(s[g * 32 + 2 * i + 1]), c, -mc));
+                        sum[i & 1] += p0, sum[2 + (i & 1)] += p1;
+                        if constexpr (SPLIT)
+                            split2(p0, p1, hi[i], lo[i]);
+                        else
+                            hi[i] = pack2(p0, p1, Part());
+                    }
+                    tmem_st16_u32(pp + q * 32 + g * 16, hi);
+                    if (SPLIT) tmem_st16_u32(pp + 32 + g * 16, lo);
+                }
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(bar(kPFull + (j & 1)));
-            if (SPLIT && j > 0) {
-                ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 22);
+            arrive(kPFull + b);
+            if (SPLIT && j > 0 && j % kSegment == 0) {
+                ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 25);
                 if (!ok) break;
                 tc_fence_after();
-                fold(j - 1);
-                if (any) {  // brought to the reference that holds from this tile on
+                columns([&](int i) {
+                    uint32_t o[16];
+                    tmem_ld16_wait(lanes + kColO + i, o);
+                    if (j > kSegment) {
+                        uint32_t r[16];
+                        tmem_ld16_wait(lanes + kColO + DCOLS + i, r);
 #pragma unroll
-                    for (int i = 0; i < (SPLIT ? DCOLS : 0); ++i) acc[SPLIT ? i : 0] *= f;
-                }
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + __uint_as_float(r[e]));
+                    }
+                    tmem_st16_u32(lanes + kColO + DCOLS + i, o);
+                });
+                tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(bar(kOEmpty + ((j - 1) & 1)));
+                arrive(kOEmpty);
             }
         }
-        if (ok && tiles > 0) ok = warp_wait(kOFull + ((tiles - 1) & 1), (tiles - 1) >> 1, 35);
+        if (ok && tiles > 0) ok = warp_wait(kOFull + ((tiles - 1) & 1), (tiles - 1) >> 1, 26);
         if (ok) {
             tc_fence_after();
-            const int64_t row = (int64_t)qb * kRows + warp * 32 + lane;
             const bool store = row < a.nq;
             const int64_t at = ((int64_t)item * a.nq + row) * a.heads + h;
-            if (SPLIT && tiles > 0) fold(tiles - 1);
             // One factor for the row: 1 / l, or for a share of the list the weights' own scale taken out.
             const float f = a.splits > 1 ? (SPLIT ? ldexpf(1.0f, -ev - kWeightExp) : 1.0f)
                                          : (l == 0.0f ? 0.0f : (SPLIT ? ldexpf(1.0f, -ev) : 1.0f) / l);
-            float* part = a.part + (at * a.splits + split) * (a.dim + 2);
+            float* part = a.part + (at * a.splits + split) * (a.dim + 4);
             if (a.splits > 1 && store) {
                 part[a.dim] = ref == -INFINITY ? ref : ref * c;
                 part[a.dim + 1] = SPLIT ? ldexpf(l, -kWeightExp) : l;
             }
+            columns([&](int i) {
+                uint32_t o[16], r[16];
+                if (tiles > 0) tmem_ld16_wait(lanes + kColO + i, o);
+                if (SPLIT && tiles > kSegment) tmem_ld16_wait(lanes + kColO + DCOLS + i, r);
 #pragma unroll
-            for (int i = 0; i < DCOLS; i += 32) {
-                uint32_t o[32];
-                if (!SPLIT && tiles > 0) tmem_ld32_wait(lanes + kColO + i, o);
-#pragma unroll
-                for (int g = 0; g < 32; g += 8) {
+                for (int g = 0; g < 16; g += 8) {
                     float y[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float v = SPLIT ? acc[SPLIT ? i + g + e : 0] : __uint_as_float(o[g + e]);
+                        float v = __uint_as_float(o[g + e]);
+                        if (SPLIT && tiles > kSegment) v += __uint_as_float(r[g + e]);
                         y[e] = l == 0.0f ? 0.0f : v * f;
                     }
                     if (!store || i + g >= a.dim) continue;
-                    if (a.splits > 1) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) part[i + g + e] = y[e];
-                    } else {
+                    if (a.splits > 1)
+                        store8(part + i + g, y);
+                    else
                         store8(static_cast<OUT*>(a.out) + at * a.dim + i + g, y);
-                    }
                 }
-            }
+            });
         }
-    } else if (warp == 4) {
+    } else if (warp != 5) {
         // ---------------------------------------------------------------- producer
         auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bytes, int full_bar, int head, int token,
                         int n_boxes, int rows) {  // one lane for each box of `rows` rows
@@ -522,17 +531,15 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             }
             __syncwarp();
         };
-        int q_done = 0, k_done = 0, v_done = 0;
-        if (!SPLIT && tiles > 0) {
-            load(&map_q, sq, PANELS * kQPanel, kQFull, h, qb * kRows, 1, kRows);
-            q_done = 1;
-        }
+        const bool is_v = warp == 6;
+        int done = 0;
+        if (!SPLIT && !is_v && tiles > 0) load(&map_q, sq, PANELS * kQPanel, kQFull, h, qb * kRows, 1, kRows);
         // The list and the mask are read ahead of the tiles that they are for: a lane holds the first token of one
-        // box (32 / boxes tiles at a time, the next ones on their way), and its two keys' mask bytes of the next tile.
+        // box (32 / boxes tiles at a time, the next ones on their way), and its keys' mask bytes of the next tile.
         const int lg_block = 31 - __clz(a.block_k), lg_rows = 31 - __clz(rows_box), lg_boxes = 31 - __clz(boxes);
         const int batch = 32 >> lg_boxes;
         auto first_token = [&](int tile) {  // of this lane's box in the batch that begins with `tile`
-            const int at = (t0 + tile) * kKeys + (lane << lg_rows), e = at >> lg_block;  // in the list's keys
+            const int at = (t0 + tile) * KEYS + (lane << lg_rows), e = at >> lg_block;  // in the list's keys
             const int blk = e < listed ? list[e] : -1;
             return (uint32_t)blk < (uint32_t)a.k_blocks ? (blk << lg_block) + (at & (a.block_k - 1))
                                                         : (int)a.nk;  // past the last key: zeros
@@ -542,58 +549,65 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         };
         int tokens = first_token(0), tokens_next = tiles > batch ? first_token(batch) : 0;
         uint32_t short_boxes = cut(tokens);
-        const uint32_t box_bits = boxes == 1 ? 1u : boxes == 2 ? 3u : 15u;
-        uint8_t keep[2] = {1, 1};
-        int64_t t_key[2] = {0, 0};
+        const uint32_t box_bits = (1u << boxes) - 1;
+        uint8_t keep[WORDS];
+        int64_t t_key[WORDS];
         bool checks = false;  // the tile's keys are looked at one by one
         auto look_up = [&](int j) {
             const int box0 = (j & (batch - 1)) << lg_boxes;
-            checks = mask || (short_boxes >> box0 & box_bits);
+            checks = is_v ? cleans : mask || (short_boxes >> box0 & box_bits);
             if (!checks) return;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < WORDS; ++i) {
                 const int key = i * 32 + lane;
                 t_key[i] = (int64_t)__shfl_sync(0xffffffffu, tokens, box0 + (key >> lg_rows)) + (key & (rows_box - 1));
-                if (mask) keep[i] = t_key[i] < a.nk ? mask[t_key[i]] : 0;
+                keep[i] = t_key[i] < a.nk && (!mask || mask[t_key[i]]);
             }
         };
         if (tiles > 0) look_up(0);
         for (int j = 0; j < tiles; ++j) {
             const int st = j % STAGES, ph = j / STAGES, slot = j % kMaskSlots;
             const int token = __shfl_sync(0xffffffffu, tokens, ((j & (batch - 1)) << lg_boxes) + (lane & (boxes - 1)));
-            uint32_t w[2] = {0xffffffffu, 0xffffffffu};
+            uint32_t w[WORDS];
             bool hidden = false;
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = 0xffffffffu;
             if (checks) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const bool in = t_key[i] < a.nk, kept = in && keep[i];
-                    w[i] = __ballot_sync(0xffffffffu, kept);
-                    hidden |= in && !kept;
+                for (int i = 0; i < WORDS; ++i) {
+                    w[i] = __ballot_sync(0xffffffffu, keep[i] != 0);
+                    hidden |= t_key[i] < a.nk && !keep[i];
                 }
                 hidden = __any_sync(0xffffffffu, hidden);
             }
-            if (j >= STAGES && !warp_wait(kKEmpty + st, ph - 1, 23)) break;
-            if (lane == 0) valid[slot][0] = w[0], valid[slot][1] = w[1];  // handed on with K, then with S
-            load(&map_k, sk + st * OP, OP, kKFull + st, kh, token, boxes, rows_box);
-            k_done = j + 1;
+            if (j >= STAGES && !warp_wait((is_v ? kVEmpty : kKEmpty) + st, ph - 1, 38)) break;
+            if (is_v) {
+                load(&map_v, sv + st * OP, OP, kVFull + st, kh, token, boxes, rows_box);
+            } else {
+                if (lane == 0) {  // handed on with K, then with S
+#pragma unroll
+                    for (int i = 0; i < WORDS; ++i) valid[slot][i] = w[i];
+                }
+                load(&map_k, sk + st * OP, OP, kKFull + st, kh, token, boxes, rows_box);
+            }
+            done = j + 1;
             if (((j + 1) & (batch - 1)) == 0) {
                 tokens = tokens_next;
                 short_boxes = cut(tokens);
                 if (j + 1 + batch < tiles) tokens_next = first_token(j + 1 + batch);
             }
             if (j + 1 < tiles) look_up(j + 1);
-            if (j >= STAGES && !warp_wait(kVEmpty + st, ph - 1, 25)) break;
-            load(&map_v, sv + st * OP, OP, kVFull + st, kh, token, boxes, rows_box);
-            v_done = j + 1;
-            if (cleans) {
+            if (is_v && cleans) {
                 if (hidden) {
-                    if (!warp_wait(kVFull + st, ph, 26)) break;
-                    for (int r = 0; r < kKeys; ++r) {
-                        if (w[r >> 5] >> (r & 31) & 1u) continue;
+                    if (!warp_wait(kVFull + st, ph, 37)) break;
 #pragma unroll
-                        for (int p = 0; p < PANELS; ++p)
-                            *reinterpret_cast<uint32_t*>(gbase + st * OP + p * kPanel + r * 128 + lane * 4) = 0;
-                    }
+                    for (int i = 0; i < WORDS; ++i)
+                        for (uint32_t gone = ~w[i]; gone; gone &= gone - 1) {
+                            const int r = i * 32 + __ffs(gone) - 1;
+#pragma unroll
+                            for (int p = 0; p < PANELS; ++p)
+                                *reinterpret_cast<uint32_t*>(gbase + st * OP + p * kPanel + r * 128 + lane * 4) = 0;
+                        }
                     fence_proxy_async_smem();
                     __syncwarp();
                 }
@@ -603,23 +617,23 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         __syncwarp();
         if (*abort_p && lane == 0) {  // copies in flight land before the CTA's memory is given up
             const long long deadline = clock64() + kWaitLimit;
-            if (q_done) drain_wait(bar(kQFull), 0, deadline, args.err, 27, kKAttention);
-            for (int i = std::max(0, k_done - STAGES); i < k_done; ++i)
-                drain_wait(bar(kKFull + i % STAGES), (uint32_t)(i / STAGES) & 1u, deadline, args.err, 27, kKAttention);
-            for (int i = std::max(0, v_done - STAGES); i < v_done; ++i)
-                drain_wait(bar(kVFull + i % STAGES), (uint32_t)(i / STAGES) & 1u, deadline, args.err, 27, kKAttention);
+            if (!SPLIT && !is_v && tiles > 0) drain_wait(bar(kQFull), 0, deadline, args.err, 40, kKAttention);
+            for (int i = std::max(0, done - STAGES); i < done; ++i)
+                drain_wait(bar((is_v ? kVFull : kKFull) + i % STAGES), (uint32_t)(i / STAGES) & 1u, deadline, args.err, 40,
+                           kKAttention);
         }
     } else if (tiles > 0) {
         // ---------------------------------------------------------------- MMA issuer
         // The whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues.
         const bool leader = elect_one();
         const int k_steps = (a.dim + 15) / 16;
-        const uint32_t idesc_s = idesc_16(BF16, kKeys, a.scale < 0.0f, false);
+        const uint32_t idesc_s = idesc_16(BF16, KEYS, a.scale < 0.0f, false);
         const uint32_t idesc_o = idesc_16(BF16, k_steps * 16, false, true);
-        const uint64_t q_desc = sw128_desc(sq), k_desc = sw128_desc(sk), v_desc = sw128_desc_mn(sv);
-        auto scores = [&](int j) {  // S of tile j, whose columns held S (and where P has none of its own, P) of tile j − 2
-            const int st = j % STAGES;
+        const uint64_t q_desc = sw128_desc(sq), k_desc = sw128_desc(sk), v_desc = sw128_desc_mn(sv, kPanel);
+        auto scores = [&](int j) {  // S of tile j, when what its columns held is used up
+            const int st = j % STAGES, b = j % NS;
             if (!warp_wait(kKFull + st, j / STAGES, 29)) return false;
+            if (OWN_P && j >= 1 && !warp_wait(kSEmpty, j - 1, 30)) return false;
             if (!OWN_P && j >= 2 && !warp_wait(kOFull + (j & 1), (j - 2) >> 1, 30)) return false;
             tc_fence_after();
             if (leader) {
@@ -630,36 +644,36 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
 #pragma unroll
                     for (int s = 0; s < 4 * PANELS; ++s)
                         if (s < k_steps)
-                            mma_16_ss(tmem + (j & 1) * kKeys, qa + ((s >> 2) * kQPanel + (s & 3) * 32 >> 4),
+                            mma_16_ss(tmem + b * KEYS, qa + ((s >> 2) * kQPanel + (s & 3) * 32 >> 4),
                                       ka + ((s >> 2) * kPanel + (s & 3) * 32 >> 4), idesc_s,
                                       (p > (SPLIT ? 0 : 2) || s > 0) ? 1u : 0u);
                 }
                 mma_commit(bar(kKEmpty + st));
-                mma_commit(bar(kSFull + (j & 1)));
-                mbar_arrive(bar(kSFull + (j & 1)));  // the producer's bits of valid keys, seen here, go on with S
+                mma_commit(bar(kSFull + b));
+                mbar_arrive(bar(kSFull + b));  // the producer's bits of valid keys, seen here, go on with S
             }
             __syncwarp();
             return true;
         };
-        bool ok = warp_wait(kQFull, 0, 28) && scores(0) && (tiles == 1 || scores(1));
+        bool ok = warp_wait(kQFull, 0, 28) && scores(0) && (NS == 1 || tiles == 1 || scores(1));
         for (int j = 0; ok && j < tiles; ++j) {
             const int st = j % STAGES, ph = j / STAGES;
-            ok = warp_wait(kPFull + (j & 1), j >> 1, 33);
-            if (ok && OWN_P && j + 2 < tiles) ok = scores(j + 2);  // tile j's S was read before its P was written
+            if (OWN_P && j + 1 < tiles) ok = scores(j + 1);
+            if (ok) ok = warp_wait(kPFull + j % NS, j / NS, 33);
             if (ok) ok = warp_wait(kVFull + st, ph, 31);
             if (ok && cleans) ok = warp_wait(kVClean + st, ph, 32);
-            if (ok && SPLIT && j >= 2) ok = warp_wait(kOEmpty + (j & 1), (j - 2) >> 1, 36);
+            if (ok && SPLIT && j > 0 && j % kSegment == 0) ok = warp_wait(kOEmpty, j / kSegment - 1, 36);
             if (!ok) break;
             tc_fence_after();
             if (leader) {
 #pragma unroll
                 for (int p = SPLIT ? 0 : 2; p < 3; ++p) {
                     const uint64_t va = v_desc + ((uint32_t)st * OP >> 4) + (p == 1 ? PANELS * kPanel >> 4 : 0);
-                    const uint32_t pa = tmem + PCOL + (j & 1) * PSTEP;
+                    const uint32_t pa = tmem + PCOL + j % NS * KEYS + (p == 0 ? 32 : 0);
 #pragma unroll
-                    for (int s = 0; s < kKeys / 16; ++s) {
-                        const bool fresh = s == 0 && (SPLIT ? p == 0 : j == 0);
-                        mma_16_ts(tmem + kColO + (SPLIT ? (j & 1) * DCOLS : 0), pa + (SPLIT ? (s >> 1) * 32 + (s & 1) * 8 + (p == 0 ? 16 : 0) : s * 8),
+                    for (int s = 0; s < KEYS / 16; ++s) {
+                        const bool fresh = s == 0 && (SPLIT ? p == 0 && j % kSegment == 0 : j == 0);
+                        mma_16_ts(tmem + kColO, pa + s * 8,
                                   va + (uint32_t)(s * 2048 >> 4), idesc_o, fresh ? 0u : 1u);
                     }
                 }
@@ -785,7 +799,7 @@ void launch_attention_tc(mbx_ctx* ctx, const AttnArgs& a, int dtype, int64_t n, 
     TcArgs t{a, nullptr, n, ctx->dev_err};
     CUtensorMap maps[3];
     const bool bf16 = dtype == MBX_DTYPE_BF16;
-    const int rows_box = std::min(a.block_k, kKeys);
+    const int rows_box = std::min(a.block_k, dtype != MBX_DTYPE_F32 && a.dim <= 64 ? keys_of<1, false>() : keys_of<2, false>());
     if (dtype == MBX_DTYPE_F32) {
         SplitArgs s{};
         const size_t amax_bytes = 4 * 2 * (size_t)(n * a.kv_heads);
