@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[kBars];
     __shared__ volatile uint32_t valid[kMaskSlots][4];
+    __shared__ uint32_t q_top[SPLIT ? kRows : 1];  // f32: bits of the query rows' largest magnitudes
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -273,13 +274,14 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t cta = blockIdx.x / a.splits;  // (item, head, query block)
+    const uint32_t cta = blockIdx.x / (uint32_t)a.splits;  // (item, head, query block)
     const int split = (int)(blockIdx.x - cta * a.splits);
-    const int qb = (int)(cta % a.q_blocks);
-    const int h = (int)(cta / a.q_blocks % a.heads);
-    const int item = (int)(cta / a.q_blocks / a.heads);
+    const uint32_t head_at = cta / (uint32_t)a.q_blocks;
+    const int qb = (int)(cta - head_at * a.q_blocks);
+    const int item = (int)(head_at / (uint32_t)a.heads);
+    const int h = (int)(head_at - (uint32_t)item * a.heads);
     const int kh = h / (a.heads / a.kv_heads);
-    const int32_t* list = a.index + cta * a.topk;
+    const int32_t* list = a.index + (int64_t)cta * a.topk;
     const uint8_t* mask = a.mask ? a.mask + (int64_t)item * a.nk : nullptr;
     const bool cleans = !SPLIT && mask != nullptr;
 
@@ -300,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         abort_flag = 0;
         fence_mbarrier_init();
     }
+    if (SPLIT && threadIdx.x < kRows) q_top[threadIdx.x] = 0;
     if (warp == 5) {
         tmem_alloc(smem_u32(&tmem_slot), TMEM);
         tmem_relinquish();
@@ -311,8 +314,8 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
     const uint32_t tmem = tmem_slot;
     const int rows_box = min(a.block_k, KEYS), boxes = KEYS / rows_box;  // TMA boxes of a tile
     const int all_tiles = (int)(((int64_t)listed * a.block_k + KEYS - 1) / KEYS);
-    const int t0 = (int)((int64_t)all_tiles * split / a.splits);
-    const int tiles = (int)((int64_t)all_tiles * (split + 1) / a.splits) - t0;
+    const int t0 = a.splits == 1 ? 0 : (int)((uint32_t)all_tiles * split / (uint32_t)a.splits);  // at most 2^17 · 64
+    const int tiles = a.splits == 1 ? all_tiles : (int)((uint32_t)all_tiles * (split + 1) / (uint32_t)a.splits) - t0;
     volatile int* abort_p = &abort_flag;
     auto wait = [&](int b, int phase, int site) {
         return mbar_wait(bar(b), (uint32_t)phase & 1u, args.err, site, abort_p, true, kWaitLimit, kKAttention);
@@ -335,34 +338,48 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         float c = fabsf(a.scale);
         int ev = 0;
         if constexpr (SPLIT) {
-            // The thread's query row in two parts, at a power of two of its own.
-            const float* x = static_cast<const float*>(a.q) + ((int64_t)item * a.nq + row) * a.q_stride + (int64_t)h * a.dim;
-            uint32_t top = 0;
-            if (row < a.nq) {
-#pragma unroll 4
-                for (int i = 0; i < a.dim; i += 8) {
-                    float v[8];
-                    widen8<float>(load_raw8(x + i), v);
+            // Q in two parts, a row at a power of two of its own. A warp reads whole rows: a lane takes pieces of eight
+            // channels, and the rows' magnitudes meet in shared memory.
+            const int pieces = a.dim >> 3, wide = (a.dim + 15) / 16 * 2;  // of a row of q; of the operand, to 16 channels
+            const float* x = static_cast<const float*>(a.q) + ((int64_t)item * a.nq + (int64_t)qb * kRows) * a.q_stride +
+                             (int64_t)h * a.dim;
+            constexpr int MOST = PANELS * 8;
+            Raw8f raw[MOST];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = larger(top, v[e]);
-                }
+            for (int k = 0; k < MOST; ++k) {
+                const int i = (int)threadIdx.x + k * kRows, r = i / wide, p = i - r * wide;
+                raw[k] = Raw8f{};
+                if (r < kRows && p < pieces && (int64_t)qb * kRows + r < a.nq)
+                    raw[k] = load_raw8(x + r * a.q_stride + p * 8);
             }
-            const int eq = scale_exponent(top);
-            const float f = ldexpf(1.0f, eq);
-            uint8_t* to = gbase + (sq - base) + threadIdx.x * 128;
-#pragma unroll 4
-            for (int i = 0; i < (a.dim + 15) / 16 * 16; i += 8) {  // a 16-byte piece, at its swizzled place
-                float v[8] = {};
-                if (row < a.nq && i < a.dim) widen8<float>(load_raw8(x + i), v);
+#pragma unroll
+            for (int k = 0; k < MOST; ++k) {
+                const int r = ((int)threadIdx.x + k * kRows) / wide;
+                float v[8];
+                widen8<float>(raw[k], v);
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = larger(top, v[e]);
+                if (r < kRows && top) atomicMax(&q_top[r], top);
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");  // the four softmax warps, none of which can have given up yet
+#pragma unroll
+            for (int k = 0; k < MOST; ++k) {
+                const int i = (int)threadIdx.x + k * kRows, r = i / wide, p = i - r * wide;
+                if (r >= kRows) continue;
+                const float f = ldexpf(1.0f, scale_exponent(q_top[r]));
+                float v[8];
+                widen8<float>(raw[k], v);
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) split2(v[2 * e] * f, v[2 * e + 1] * f, hi[e], lo[e]);
-                const int at = (i >> 6) * (int)kQPanel + (((i >> 3) & 7) ^ (threadIdx.x & 7)) * 16;
-                *reinterpret_cast<uint4*>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(to + at + PANELS * kQPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                uint8_t* to = gbase + (sq - base) + (p >> 3) * kQPanel + r * 128 + ((p & 7) ^ (r & 7)) * 16;  // swizzled
+                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(to + PANELS * kQPanel) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
             fence_proxy_async_smem();
             arrive(kQFull);
+            const int eq = scale_exponent(q_top[threadIdx.x]);
             const uint32_t* kv = args.amax + (int64_t)item * a.kv_heads + kh;
             ev = part_exponent(kv[args.n * a.kv_heads]);
             c = ldexpf(c, -(eq + part_exponent(*kv)));
