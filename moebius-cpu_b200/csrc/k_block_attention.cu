@@ -4,11 +4,14 @@
 // over the keys j of the blocks that index[b, h, r / 128] lists and that the
 // key mask keeps; a row without any such key is zero.
 //
-// The rows kernel: one pass over the listed keys with a running maximum and sum (f32). A group of
-// lanes holds one key's channels, eight a lane, so a warp works on several keys at a time; every
-// group keeps its own maximum, sum and output for R query rows and the groups and warps are joined
-// at the end. Where there are few rows the listed blocks are split over several CTAs, whose partial
-// (output, maximum, sum) a second kernel joins.
+// Many query rows go to the tensor cores (k_block_attention_tc.cu); this file has the kernel for few rows, the one
+// that joins split lists, and the choice between them.
+//
+// The rows kernel reads every listed key and value once for R query rows and is bound by that. A group
+// of dim / 8 lanes holds one key's channels, eight a lane, so a warp works on several keys at a time, and
+// U keys of a group are on their way together. Every group keeps its own running maximum, sum and
+// output (f32); groups and warps are joined at the end through shared memory. A list is split over
+// CTAs, and a second kernel joins their partial (output, maximum, sum).
 #include <algorithm>
 
 #include "block_attention.h"
@@ -19,29 +22,43 @@ namespace mbx {
 namespace {
 
 constexpr int kRowWarps = 4;
+constexpr int kListPart = 1024;  // list entries in shared memory at a time
+
+// Loads that stay where they are written: left to itself the compiler moves a value's load behind the dot products.
+__device__ __forceinline__ void load_now(uint4& r, const void* p) {
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+}
+__device__ __forceinline__ void load_now(Raw8f& r, const float* p) {
+    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(r.a.x), "=f"(r.a.y), "=f"(r.a.z), "=f"(r.a.w) : "l"(p));
+    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(r.b.x), "=f"(r.b.y), "=f"(r.b.z), "=f"(r.b.w)
+                 : "l"(p + 4));
+}
 
 // Lanes of a key's group: the power of two that holds dim / 8.
-template <class T, int R>
-__global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const AttnArgs a, int group) {
-    // One slot per (warp, group, row) and then the join: maxima, sums, outputs.
+template <class T, int R, int U>
+__global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const AttnArgs a, int lg_group) {
+    // One slot per (warp, group, row) for the join at the end: maxima, sums, outputs.
     extern __shared__ float sh[];
+    __shared__ int list[kListPart];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int li = lane & (group - 1), gi = lane / group, groups = 32 / group;
+    const int group = 1 << lg_group, li = lane & (group - 1), gi = lane >> lg_group, groups = 32 >> lg_group;
     const int slots = kRowWarps * groups, slot = warp * groups + gi;
     const bool holds = li * 8 < a.dim;
-    const int tiles = (int)((a.nq + R - 1) / R);
-    const int64_t cta = blockIdx.x / a.splits;
+    const uint32_t tiles = (uint32_t)((a.nq + R - 1) / R);
+    const uint32_t cta = blockIdx.x / (uint32_t)a.splits, head_at = cta / tiles;
     const int split = (int)(blockIdx.x - cta * a.splits);
-    const int64_t r0 = cta % tiles * R;
-    const int h = (int)(cta / tiles % a.heads);
-    const int64_t item = cta / tiles / a.heads;
-    const int kh = h / (a.heads / a.kv_heads);
+    const int64_t r0 = (int64_t)(cta - head_at * tiles) * R;
+    const int64_t item = head_at / (uint32_t)a.heads;
+    const int h = (int)(head_at - (uint32_t)item * a.heads), kh = h / (a.heads / a.kv_heads);
     // A tile of R rows never straddles two query blocks: R divides 128.
-    const int32_t* list = a.index + ((item * a.heads + h) * a.q_blocks + r0 / MBX_ATTENTION_BLOCK_Q) * a.topk;
+    const int32_t* index = a.index + ((item * a.heads + h) * a.q_blocks + r0 / MBX_ATTENTION_BLOCK_Q) * a.topk;
     const T* q = static_cast<const T*>(a.q) + (item * a.nq + r0) * a.q_stride + (int64_t)h * a.dim + li * 8;
-    const T* k = static_cast<const T*>(a.k) + item * a.nk * a.k_stride + (int64_t)kh * a.dim + li * 8;
-    const T* v = static_cast<const T*>(a.v) + item * a.nk * a.v_stride + (int64_t)kh * a.dim + li * 8;
+    const T* k0 = static_cast<const T*>(a.k) + item * a.nk * a.k_stride + (int64_t)kh * a.dim;
+    const T* v0 = static_cast<const T*>(a.v) + item * a.nk * a.v_stride + (int64_t)kh * a.dim;
+    const T *k = k0 + li * 8, *v = v0 + li * 8;
     const uint8_t* mask = a.mask ? a.mask + item * a.nk : nullptr;
+    const int lg_block = 31 - __clz(a.block_k);
 
     float qv[R][8], acc[R][8] = {}, m[R], l[R];
 #pragma unroll
@@ -54,50 +71,90 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const At
         for (int i = 0; i < 8; ++i) qv[r][i] *= a.scale;
     }
 
-    const int64_t first = a.topk * split / a.splits, last = a.topk * (split + 1) / a.splits;
-    for (int64_t e = first; e < last; ++e) {
-        const int blk = list[e];
-        if (blk < 0 || blk >= a.k_blocks) continue;
-        const int64_t j0 = (int64_t)blk * a.block_k;
-        const int keys = (int)min((int64_t)a.block_k, a.nk - j0);
-        for (int s = slot; s - gi - warp * groups < keys; s += slots) {  // the same trips in every lane of the block
-            const int64_t j = j0 + s;
-            const bool on = s < keys && (!mask || mask[j]);
-            float kv[8] = {}, vv[8] = {};
-            if (on && holds) {
-                widen8<T>(load_raw8(k + j * a.k_stride), kv);
-                widen8<T>(load_raw8(v + j * a.v_stride), vv);
+    const int first = (int)(a.topk * split / a.splits), last = (int)(a.topk * (split + 1) / a.splits);
+    using Raw = typename Raw8<T>::type;
+    for (int part = first; part < last; part += kListPart) {
+        const int entries = min(kListPart, last - part);
+        __syncthreads();
+        for (int e = threadIdx.x; e < entries; e += kRowWarps * 32) list[e] = index[part + e];
+        __syncthreads();
+        const int64_t end = (int64_t)entries << lg_block;  // in the list's keys
+        for (int64_t p0 = (int64_t)warp * U * groups; p0 < end; p0 += (int64_t)kRowWarps * U * groups) {
+            Raw kr[U], vr[U];
+            bool on[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t p = p0 + u * groups + gi;
+                const int blk = p < end ? list[p >> lg_block] : -1;
+                const int64_t j = ((int64_t)blk << lg_block) + (p & (a.block_k - 1));
+                on[u] = (uint32_t)blk < (uint32_t)a.k_blocks && j < a.nk && (!mask || mask[j]);
+                // Every lane loads, from the item's first key where it has none, so that all loads are under way at once.
+                const bool real = on[u] && holds;
+                load_now(kr[u], real ? k + j * a.k_stride : k0);
+                load_now(vr[u], real ? v + j * a.v_stride : v0);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (!(on[u] && holds)) kr[u] = Raw{}, vr[u] = Raw{};
+            float d[U][R];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float kv[8];
+                widen8<T>(kr[u], kv);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    d[u][r] = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d[u][r] = fmaf(qv[r][i], kv[i], d[u][r]);
+                }
+            }
+            for (int o = group >> 1; o > 0; o >>= 1) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) d[u][r] += __shfl_xor_sync(0xffffffffu, d[u][r], o);
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float d = 0.0f;
+                float mn = m[r];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d = fmaf(qv[r][i], kv[i], d);
-                for (int o = group >> 1; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-                if (on && d != -INFINITY) {
-                    const float mn = fmaxf(m[r], d);
-                    const float c = exp2f(m[r] - mn), p = exp2f(d - mn);
-                    m[r] = mn;
-                    l[r] = l[r] * c + p;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[r][i] = fmaf(acc[r][i], c, p * vv[i]);
+                for (int u = 0; u < U; ++u) {
+                    if (!on[u]) d[u][r] = -INFINITY;
+                    mn = fmaxf(mn, d[u][r]);
                 }
+                const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing yet: every weight is 2^-inf
+                const float c = exp2f(m[r] - ref);
+                m[r] = mn, l[r] *= c;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[r][i] *= c;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    d[u][r] = exp2f(d[u][r] - ref);
+                    l[r] += d[u][r];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float vv[8];
+                widen8<T>(vr[u], vv);
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[r][i] = fmaf(d[u][r], vv[i], acc[r][i]);
             }
         }
     }
 
-    float* sm = sh;                  // [slots][R]
-    float* sl = sm + slots * R;      // [slots][R]
-    float* so = sl + slots * R;      // [slots][R][dim]
+    float* sm = sh;              // [slots][R]
+    float* sl = sm + slots * R;  // [slots][R]
+    float* so = sl + slots * R;  // [slots][R][dim]
     if (li == 0) {
 #pragma unroll
         for (int r = 0; r < R; ++r) sm[slot * R + r] = m[r], sl[slot * R + r] = l[r];
     }
     if (holds) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) so[(slot * R + r) * a.dim + li * 8 + i] = acc[r][i];
+        for (int r = 0; r < R; ++r) store8(so + (slot * R + r) * a.dim + li * 8, acc[r]);
     }
     __syncthreads();
     for (int e = threadIdx.x; e < R * a.dim; e += kRowWarps * 32) {
@@ -105,10 +162,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const At
         if (r0 + r >= a.nq) continue;
         float top = -INFINITY;
         for (int s = 0; s < slots; ++s) top = fmaxf(top, sm[s * R + r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
         float sum = 0.0f, o = 0.0f;
+#pragma unroll 4
         for (int s = 0; s < slots; ++s) {
-            const float ms = sm[s * R + r];
-            const float w = ms == -INFINITY ? 0.0f : exp2f(ms - top);
+            const float w = exp2f(sm[s * R + r] - ref);
             sum = fmaf(w, sl[s * R + r], sum);
             o = fmaf(w, so[(s * R + r) * a.dim + ch], o);
         }
@@ -132,6 +190,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a) {
     __shared__ float weight[kMaxSplits];
     __shared__ float4 acc[4][32];
     __shared__ float total;
+    cudaGridDependencySynchronize();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stride = a.dim + 4;
     const float* p = a.part + (int64_t)blockIdx.x * a.splits * stride;
     if (warp == 0) {
@@ -173,49 +232,65 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a) {
     }
 }
 
-constexpr int kRowsR = 4;
 constexpr int64_t kSms = 148;
 
-// Which kernel takes a problem, and over how many CTAs a list is split: enough to fill the card
-// twice over, never more than there are blocks (rows) or tiles of 64 keys (tensor cores).
+// Which kernel takes a problem, and over how many CTAs a list is split.
 struct Plan {
-    bool rows;
+    int rows;  // query rows of a CTA of the rows kernel; 0: the tensor cores
     int splits;
     size_t part_bytes, split_bytes;
 };
 
 Plan plan_of(const BlockShape& s, int64_t topk) {
     Plan p{};
-    p.rows = s.dtype == MBX_DTYPE_F32 && s.nq < 16;
-    const int64_t tile = p.rows ? kRowsR : MBX_ATTENTION_BLOCK_Q;
+    // 16 bits: the rows kernel for one or two rows of few heads (16 heads x 128 over 4096 of 65536 keys bf16: 14 us against
+    // 21, four rows 29 against 21; 128 heads: 72 us against 63). f32: while it reads no more than twice the keys that the tensor cores' operands would have to
+    // be split for (the same shape, 32 rows: 141 us against 238, 64: 240 against 240; 16 x 1024 of 4096 keys x 8 x 40, 32
+    // rows: 100 against 108, 64: 190 against 112).
+    const bool few = s.dtype == MBX_DTYPE_F32
+                         ? (s.nq + 3) / 4 * s.heads * std::min(topk * s.block_k, s.nk) <= 2 * s.nk * s.kv_heads
+                         : s.nq <= 2 && s.n * s.heads < 64;
+    if (few) p.rows = s.nq == 1 ? 1 : s.nq == 2 ? 2 : 4;
+    // Enough CTAs to fill the card four times over (rows) or twice (tensor cores), with equal shares of the list's blocks
+    // or tiles of 64 keys.
+    const int64_t tile = p.rows ? p.rows : MBX_ATTENTION_BLOCK_Q;
     const int64_t ctas = std::max<int64_t>(1, s.n * s.heads * ((s.nq + tile - 1) / tile));
-    const int64_t pieces = p.rows ? topk : (topk * s.block_k + 63) / 64;
-    p.splits = (int)std::max<int64_t>(1, std::min({(2 * kSms + ctas - 1) / ctas, pieces, int64_t(kMaxSplits)}));
+    const int64_t pieces = std::max<int64_t>(1, p.rows ? topk : (topk * s.block_k + 63) / 64);
+    const int64_t want = std::min(((p.rows ? 4 : 2) * kSms + ctas - 1) / ctas, int64_t(kMaxSplits));
+    const int64_t share = (pieces + want - 1) / want;
+    p.splits = (int)((pieces + share - 1) / share);
     if (p.splits > 1)
         p.part_bytes = align256(sizeof(float) * (size_t)(s.n * s.nq * s.heads) * p.splits * (s.dim + 4));
     if (!p.rows && s.dtype == MBX_DTYPE_F32) p.split_bytes = attention_split_bytes(s);
     return p;
 }
 
-template <class T>
+template <class T, int R>
 void launch_rows(mbx_ctx* ctx, const AttnArgs& a, int64_t n) {
-    int group = 1;
-    while (group * 8 < a.dim) group *= 2;
-    const int slots = kRowWarps * (32 / group);
-    const size_t smem = sizeof(float) * (size_t)slots * kRowsR * (a.dim + 2);
-    const int64_t ctas = n * a.heads * ((a.nq + kRowsR - 1) / kRowsR) * a.splits;
+    int lg_group = 0;
+    while ((8 << lg_group) < a.dim) ++lg_group;
+    const int slots = kRowWarps * (32 >> lg_group);
+    const size_t smem = sizeof(float) * (size_t)slots * R * (a.dim + 2);
+    const int64_t ctas = n * a.heads * ((a.nq + R - 1) / R) * a.splits;
     MBX_REQUIRE(ctas < (int64_t(1) << 31), "block_attention: too many query rows");
-    ensure_smem_limit((const void*)attention_rows_kernel<T, kRowsR>, (int)smem, "attention_rows");
-    attention_rows_kernel<T, kRowsR><<<(unsigned)ctas, kRowWarps * 32, smem, ctx->stream>>>(a, group);
+    constexpr int U = (sizeof(T) == 2 ? 4 : 2) * (R == 1 ? 2 : 1);  // 128 bytes of keys and values a lane, 256 for one row
+    ensure_smem_limit((const void*)attention_rows_kernel<T, R, U>, (int)smem, "attention_rows");
+    attention_rows_kernel<T, R, U><<<(unsigned)ctas, kRowWarps * 32, smem, ctx->stream>>>(a, lg_group);
     after_launch(ctx, "attention_rows");
+}
+
+template <class T>
+void launch_rows_any(mbx_ctx* ctx, const AttnArgs& a, int64_t n, int rows) {
+    if (rows == 1) return launch_rows<T, 1>(ctx, a, n);
+    if (rows == 2) return launch_rows<T, 2>(ctx, a, n);
+    launch_rows<T, 4>(ctx, a, n);
 }
 
 template <class T>
 void launch_join(mbx_ctx* ctx, const AttnArgs& a, int64_t n) {
     const int64_t rows = n * a.nq * a.heads;
     MBX_REQUIRE(rows < (int64_t(1) << 31), "block_attention: too many query rows");
-    attention_join_kernel<T><<<(unsigned)rows, 128, 0, ctx->stream>>>(a);
-    after_launch(ctx, "attention_join");
+    launch_after(ctx, "attention_join", attention_join_kernel<T>, dim3((unsigned)rows), 128, 0, a);
 }
 
 }  // namespace
@@ -241,10 +316,16 @@ void launch_block_attention(mbx_ctx* ctx, const BlockShape& s, const void* q, in
     a.out = out;
     a.part = static_cast<float*>(workspace);
     a.splits = p.splits;
-    if (p.rows)
-        launch_rows<float>(ctx, a, s.n);
-    else
+    if (p.rows) {
+        if (s.dtype == MBX_DTYPE_F32)
+            launch_rows_any<float>(ctx, a, s.n, p.rows);
+        else if (s.dtype == MBX_DTYPE_F16)
+            launch_rows_any<__half>(ctx, a, s.n, p.rows);
+        else
+            launch_rows_any<__nv_bfloat16>(ctx, a, s.n, p.rows);
+    } else {
         launch_attention_tc(ctx, a, s.dtype, s.n, static_cast<uint8_t*>(workspace) + p.part_bytes);
+    }
     if (p.splits == 1) return;
     if (s.dtype == MBX_DTYPE_F32) return launch_join<float>(ctx, a, s.n);
     if (s.dtype == MBX_DTYPE_F16) return launch_join<__half>(ctx, a, s.n);

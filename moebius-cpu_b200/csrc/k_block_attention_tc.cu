@@ -771,6 +771,7 @@ __global__ void __launch_bounds__(kSplitThreads) attention_split_kernel(const __
 
 // The heads that the fixed exponent does not fit, once more with their own.
 __global__ void __launch_bounds__(kSplitThreads) attention_resplit_kernel(const __grid_constant__ SplitArgs a) {
+    cudaGridDependencySynchronize();
     const int64_t total = 2 * a.n * a.heads;
     bool none = true;
     for (int64_t i = threadIdx.x; i < total; i += kSplitThreads) none &= fixed_fits(a.amax[i]);
@@ -832,8 +833,7 @@ void launch_attention_tc(mbx_ctx* ctx, const AttnArgs& a, int dtype, int64_t n, 
                         (unsigned)(2 * ((a.kv_heads * a.dim / 8 + 31) / 32)), (unsigned)n);
         attention_split_kernel<<<grid, kSplitThreads, 0, ctx->stream>>>(s);
         after_launch(ctx, "attention_split");
-        attention_resplit_kernel<<<ctx->sm_count, kSplitThreads, 0, ctx->stream>>>(s);
-        after_launch(ctx, "attention_resplit");
+        launch_after(ctx, "attention_resplit", attention_resplit_kernel, dim3((unsigned)ctx->sm_count), kSplitThreads, 0, s);
         t.amax = s.amax;
         for (int i = 1; i < 3; ++i)
             encode_heads(&maps[i], s.parts[i - 1], false, 2 * n, a.nk, a.kv_heads, a.dim, (int64_t)a.kv_heads * a.dim,

@@ -144,6 +144,7 @@ __device__ __forceinline__ void mma_f64(double (&c)[4], const double (&a)[2], do
 template <int WI, int WJ>
 __global__ void __launch_bounds__(kScoreThreads, 4) block_scores_kernel(const ScoreArgs a) {
     constexpr int TI = 2 * WI, TJ = 2 * WJ, MI = WI / 16, NJ = WJ / 8;
+    cudaGridDependencySynchronize();
     // 20 values a row of 16: four channels of four rows fall into different banks.
     constexpr int ROW = kSK + 4;
     __shared__ __align__(16) double qs[2][TI][ROW], ks[2][TJ][ROW];
@@ -229,6 +230,7 @@ template <int N>
 __global__ void __launch_bounds__(kTopWarps * 32) block_topk_kernel(const uint64_t* __restrict__ keys, int64_t rows,
                                                                     int k_blocks, int64_t topk,
                                                                     int32_t* __restrict__ index) {
+    cudaGridDependencySynchronize();
     const int64_t row = blockIdx.x * (int64_t)kTopWarps + (threadIdx.x >> 5);
     if (row >= rows) return;
     const int lane = threadIdx.x & 31;
@@ -357,9 +359,8 @@ SelectLayout select_layout(const BlockShape& s) {
 
 template <int N>
 void launch_topk(mbx_ctx* ctx, const uint64_t* keys, int64_t rows, int kb, int64_t topk, int32_t* index) {
-    block_topk_kernel<N><<<(unsigned)((rows + kTopWarps - 1) / kTopWarps), kTopWarps * 32, 0, ctx->stream>>>(
-        keys, rows, kb, topk, index);
-    after_launch(ctx, "block_topk");
+    launch_after(ctx, "block_topk", block_topk_kernel<N>, dim3((unsigned)((rows + kTopWarps - 1) / kTopWarps)), kTopWarps * 32,
+                 0, keys, rows, kb, topk, index);
 }
 
 }  // namespace
@@ -389,10 +390,11 @@ void launch_block_select(mbx_ctx* ctx, const BlockShape& s, const void* q, int64
                      kb};
         const unsigned z = (unsigned)(s.n * s.heads);
         if ((int64_t)z * ((qb + 63) / 64) * ((kb + 63) / 64) >= 4 * (int64_t)ctx->sm_count)
-            block_scores_kernel<32, 32><<<dim3((kb + 63) / 64, (qb + 63) / 64, z), kScoreThreads, 0, ctx->stream>>>(sc);
+            launch_after(ctx, "block_scores", block_scores_kernel<32, 32>, dim3((kb + 63) / 64, (qb + 63) / 64, z), kScoreThreads,
+                         0, sc);
         else
-            block_scores_kernel<16, 16><<<dim3((kb + 31) / 32, (qb + 31) / 32, z), kScoreThreads, 0, ctx->stream>>>(sc);
-        after_launch(ctx, "block_scores");
+            launch_after(ctx, "block_scores", block_scores_kernel<16, 16>, dim3((kb + 31) / 32, (qb + 31) / 32, z), kScoreThreads,
+                         0, sc);
     }
     const int64_t rows = s.n * s.heads * qb;
     if (kb <= 64) return launch_topk<2>(ctx, keys, rows, kb, topk, index);
