@@ -775,7 +775,7 @@ int32_t mbx_qkv_norm_rope(mbx_ctx* ctx, const void* x, int32_t x_dtype, int64_t 
                           int32_t out_dtype) {
     return guard([&] {
         require_ctx(ctx);
-        MBX_REQUIRE(n >= 0 && tokens >= 0 && n < kMaxExtent && tokens < kMaxExtent && n * tokens < (int64_t(1) << 34),
+        MBX_REQUIRE(n >= 0 && tokens >= 0 && n < kMaxExtent && tokens < kMaxExtent && n * tokens < kMaxExtent,
                     "bad shape");
         MBX_REQUIRE(heads >= 0 && kv_heads >= 0 && heads + kv_heads > 0 && heads <= 65536 && kv_heads <= 65536,
                     "bad head counts");
