@@ -363,6 +363,12 @@ def matmul(a: DeviceTensor, b: DeviceTensor, c: Optional[DeviceTensor] = None,
     return c
 
 
+# These calls are made per layer and step, some of them shorter than a microsecond of Python: addresses go to ctypes as
+# plain integers and types are compared as the dtype objects they are.
+_F32, _I32, _U8 = np.dtype(np.float32), np.dtype(np.int32), np.dtype(np.uint8)
+_Int64x3 = ctypes.c_int64 * 3
+
+
 def _storage(t: DeviceTensor) -> int:
     code = _STORAGE.get(t.dtype)
     if code is None:
@@ -370,10 +376,18 @@ def _storage(t: DeviceTensor) -> int:
     return code
 
 
-def _fits(t: Optional[DeviceTensor], shape: tuple, dtype, what: str) -> None:
+def _fits(t: DeviceTensor, shape: tuple, dtype: np.dtype, what: str) -> None:
     """A tensor of the caller's holds what a kernel reads or writes there."""
-    if t is not None and (t.shape != shape or t.dtype != dtype):
+    if t.shape != shape or (t.dtype is not dtype and t.dtype != dtype):
         raise ValueError(f"{what} must be {dtype} of shape {shape}, not {t.dtype} of {t.shape}")
+
+
+def _at(t: Optional[DeviceTensor], shape: tuple, dtype: np.dtype, what: str) -> Optional[int]:
+    """The address of a tensor that may be left out."""
+    if t is None:
+        return None
+    _fits(t, shape, dtype, what)
+    return t.ptr
 
 
 def qkv_norm_rope(x: DeviceTensor, heads: int, kv_heads: int, dim: int, positions: Optional[DeviceTensor] = None,
@@ -390,29 +404,32 @@ def qkv_norm_rope(x: DeviceTensor, heads: int, kv_heads: int, dim: int, position
         out = (x.ctx.empty((n, tokens, heads, dim), dtype), x.ctx.empty((n, tokens, kv_heads, dim), dtype),
                x.ctx.empty((n, tokens, kv_heads, dim), dtype))
     q, k, v = out
-    kind = next(t for t in out if t is not None).dtype
-    for t, h, what in ((q, heads, "q"), (k, kv_heads, "k"), (v, kv_heads, "v")):
-        _fits(t, (n, tokens, h, dim), kind, what)
-    for t, what in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
-        _fits(t, (dim,), np.float32, what)
-    items = 1
+    kind = (q or k or v).dtype
+    q_at, k_at, v_at = (_at(t, (n, tokens, h, dim), kind, what)
+                        for t, h, what in ((q, heads, "q"), (k, kv_heads, "k"), (v, kv_heads, "v")))
+    items, positions_at = 1, None
     if positions is not None:
         items = positions.shape[0] if len(positions.shape) == 3 else 1
-        _fits(positions, (items,) * (len(positions.shape) - 2) + (tokens, 3), np.float32, "positions")
-    check(lib().mbx_qkv_norm_rope(x.ctx.handle, x.vp, _storage(x), n, tokens, stride, heads, kv_heads, dim, int(norm),
-                                  _vp(q_gamma), _vp(k_gamma), eps, _vp(positions), items,
-                                  (ctypes.c_int64 * 3)(*axis_dims), theta, PAIRINGS[pairing], _vp(q), _vp(k), _vp(v),
-                                  _STORAGE.get(kind, -1)))
+        positions_at = _at(positions, (items,) * (len(positions.shape) - 2) + (tokens, 3), _F32, "positions")
+    check(lib().mbx_qkv_norm_rope(x.ctx.handle, x.ptr, _storage(x), n, tokens, stride, heads, kv_heads, dim, norm,
+                                  _at(q_gamma, (dim,), _F32, "q_gamma"), _at(k_gamma, (dim,), _F32, "k_gamma"), eps,
+                                  positions_at, items, _Int64x3(*axis_dims), theta, PAIRINGS[pairing], q_at, k_at,
+                                  v_at, _STORAGE.get(kind, -1)))
     return out
 
 
 def _heads(q: DeviceTensor, k: DeviceTensor):
     """(n, nq, nk, heads, kv_heads, dim) of token-major head tensors."""
-    if len(q.shape) != 4 or len(k.shape) != 4 or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+    try:
+        n, nq, heads, dim = q.shape
+        kn, nk, kv_heads, k_dim = k.shape
+    except ValueError:
+        n, kn = 0, 1
+    if n != kn or dim != k_dim:
         raise ValueError("expected q [n, nq, heads, dim] and k [n, nk, kv_heads, dim]")
-    if q.dtype != k.dtype:
+    if q.dtype is not k.dtype and q.dtype != k.dtype:
         raise ValueError("q and k differ in type")
-    return q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3]
+    return n, nq, nk, heads, kv_heads, dim
 
 
 def _scratch(ctx: Context, nbytes: int) -> DeviceTensor:
@@ -435,12 +452,12 @@ def block_select(q: DeviceTensor, k: DeviceTensor, topk: int, block_k: int = 64,
     n, nq, nk, heads, kv_heads, dim = _heads(q, k)
     shape = (n, heads, -(-nq // abi.ATTENTION_BLOCK_Q), topk)
     out = out or q.ctx.empty(shape, np.int32)
-    _fits(out, shape, np.int32, "out")
-    _fits(key_mask, (n, nk), np.uint8, "key_mask")
+    _fits(out, shape, _I32, "out")
+    mask_at = _at(key_mask, (n, nk), _U8, "key_mask")
     workspace = workspace or block_select_workspace(q, k, block_k)
-    check(lib().mbx_block_select(q.ctx.handle, q.vp, heads * dim if q_stride is None else q_stride, k.vp,
+    check(lib().mbx_block_select(q.ctx.handle, q.ptr, heads * dim if q_stride is None else q_stride, k.ptr,
                                  kv_heads * dim if k_stride is None else k_stride, _storage(q), n, nq, nk, heads,
-                                 kv_heads, dim, block_k, _vp(key_mask), topk, out.vp, workspace.vp, workspace.nbytes))
+                                 kv_heads, dim, block_k, mask_at, topk, out.ptr, workspace.ptr, workspace.nbytes))
     return out
 
 
@@ -460,18 +477,19 @@ def block_attention(q: DeviceTensor, k: DeviceTensor, v: DeviceTensor, index: De
     """softmax(scale q k^T) v over the key blocks that index lists for each 128 query rows (mbx_block_attention);
     scale is 1 / sqrt(dim) by default."""
     n, nq, nk, heads, kv_heads, dim = _heads(q, k)
+    topk = index.shape[-1]
     _fits(v, k.shape, k.dtype, "v")
-    _fits(index, (n, heads, -(-nq // abi.ATTENTION_BLOCK_Q)) + index.shape[-1:], np.int32, "index")
-    _fits(key_mask, (n, nk), np.uint8, "key_mask")
+    _fits(index, (n, heads, -(-nq // abi.ATTENTION_BLOCK_Q), topk), _I32, "index")
+    mask_at = _at(key_mask, (n, nk), _U8, "key_mask")
     out = out or q.ctx.empty(q.shape, q.dtype)
     _fits(out, q.shape, q.dtype, "out")
     workspace = workspace or block_attention_workspace(q, k, index, block_k)
     kv_row = kv_heads * dim
-    check(lib().mbx_block_attention(q.ctx.handle, q.vp, heads * dim if q_stride is None else q_stride, k.vp,
-                                    kv_row if k_stride is None else k_stride, v.vp,
+    check(lib().mbx_block_attention(q.ctx.handle, q.ptr, heads * dim if q_stride is None else q_stride, k.ptr,
+                                    kv_row if k_stride is None else k_stride, v.ptr,
                                     kv_row if v_stride is None else v_stride, _storage(q), n, nq, nk, heads, kv_heads,
-                                    dim, block_k, _vp(key_mask), index.vp, index.shape[-1],
-                                    1.0 / math.sqrt(dim) if scale is None else scale, out.vp, workspace.vp,
+                                    dim, block_k, mask_at, index.ptr, topk,
+                                    1.0 / math.sqrt(dim) if scale is None else scale, out.ptr, workspace.ptr,
                                     workspace.nbytes))
     return out
 
