@@ -451,6 +451,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             if (OWN_P && j > 0) {  // P of the last tile has been read
                 ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 23);
                 if (!ok) break;
+                tc_fence_after();
             }
             const float mc = (ref == -INFINITY ? 0.0f : ref) * c - (SPLIT ? (float)kWeightExp : 0.0f);
             float sum[4] = {};

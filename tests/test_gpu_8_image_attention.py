@@ -177,7 +177,9 @@ ATTEND = [  # n, nq, nk, heads, kv_heads, dim, block_k, topk, mask
     (1, 129, 513, 2, 2, 80, 128, 3, "hole"), (3, 200, 1000, 4, 4, 16, 64, 5, "empty"),
     (1, 400, 2000, 6, 2, 128, 64, 16, "none"), (2, 300, 700, 2, 1, 72, 32, 13, "hole"),
     (1, 1030, 1030, 1, 1, 120, 16, 20, "hole"), (1, 513, 4096, 2, 2, 64, 128, 32, "none"),
-    (1, 5, 300, 1, 1, 56, 16, 25, "none")]
+    (1, 5, 300, 1, 1, 56, 16, 25, "none"), (1, 130, 200, 1, 1, 8, 16, 5, "none"), (2, 260, 999, 3, 3, 24, 32, 31, "hole"),
+    (1, 129, 300, 2, 1, 104, 64, 9, "empty"), (1, 130, 20000, 1, 1, 16, 16, 1100, "none"),
+    (1, 1, 20000, 1, 1, 16, 16, 1100, "hole")]
 
 
 def attend_inputs(rng, n, nq, nk, heads, kv, dim, block_k, topk, how, kind):
@@ -265,6 +267,54 @@ def test_block_attention_of_small_and_large_values(mbx, ctx, kind, size):
     out = mbx.block_attention(*(up(ctx, t) for t in (q, k, v, index)), block_k=32, scale=0.2 / size)
     want, tol = ref.attention(*(ref.wide(t) for t in (q, k, v)), index, 32, None, 0.2 / size, kind)
     close(out.numpy(), want, tol)
+
+
+def test_block_attention_long_list_of_one_token(mbx, ctx):
+    """More list entries for one CTA than it keeps in shared memory at a time."""
+    rng = np.random.default_rng(31)
+    heads, blocks, dim = 40, 12000, 8
+    q, k, v = (ref.narrow(rng.standard_normal((1, t, h, dim)), "f16") for t, h in
+               ((1, heads), (blocks * 16, 1), (blocks * 16, 1)))
+    index = np.broadcast_to(np.arange(blocks, dtype=np.int32), (1, heads, 1, blocks)).copy()
+    index[0, :, 0, 5000:7000] = -1
+    out = mbx.block_attention(*(up(ctx, t) for t in (q, k, v, index)), block_k=16)
+    wide = [ref.wide(t) for t in (q, k, v)]
+    kept = np.r_[0:5000 * 16, 7000 * 16:blocks * 16]
+    p = np.exp(wide[0][0, 0] @ wide[1][0, kept, 0].T * dim ** -0.5)
+    total = p.sum(1, keepdims=True)
+    want, spread = p @ wide[2][0, kept, 0] / total, p @ np.abs(wide[2][0, kept, 0]) / total
+    # f32 throughout: at most 12000 roundings of 2^-24 in a lane's sums, 2^-17 for logits and exponentials.
+    tol = (12000 * 2.0 ** -24 + 2.0 ** -17) * spread
+    close(out.numpy()[0, 0], want, tol + ref.HALF_STEP["f16"] * (np.abs(want) + tol))
+
+
+@pytest.mark.parametrize("kind,nq", [("f32", 1), ("f16", 1), ("bf16", 200)])
+def test_offsets_past_32_bits(mbx, ctx, kind, nq):
+    """Keys and values in rows of 1024 elements, over two million tokens on: element offsets past 2^31."""
+    rng = np.random.default_rng(37)
+    row, dim, nk, last = 1024, 64, 2_200_000, 3
+    step = ref.KINDS[kind].itemsize
+    big = ctx.alloc(nk * row * step)
+    try:
+        block = 64
+        first = nk // block - last  # the last full blocks
+        kv = [ref.narrow(rng.standard_normal((last * block, dim)), kind) for _ in range(2)]
+        rows = np.zeros((last * block, row), ref.KINDS[kind])
+        rows[:, 128:128 + dim], rows[:, 512:512 + dim] = kv
+        at = big + first * block * row * step
+        mbx.check(mbx.abi.lib().mbx_memcpy_h2d(ctx.handle, at, rows.ctypes.data_as(ctypes.c_void_p), rows.nbytes))
+        ctx.synchronize()
+        q = ref.narrow(rng.standard_normal((1, nq, 1, dim)), kind)
+        k, v = (mbx.DeviceTensor.wrap(ctx, big + c * step, (1, nk, 1, dim), ref.KINDS[kind]) for c in (128, 512))
+        index = np.broadcast_to(np.arange(first, first + last, dtype=np.int32), (1, 1, -(-nq // 128), last)).copy()
+        out = mbx.block_attention(up(ctx, q), k, v, up(ctx, index), k_stride=row, v_stride=row)
+        want, tol = ref.attention(ref.wide(q), *(ref.wide(t)[None, :, None] for t in kv), index - first, 64, None,
+                                  dim ** -0.5, kind)
+        close(out.numpy(), want, tol)
+    finally:
+        ctx.synchronize()
+        ctx.free(big)
+        ctx.release_below(1 << 62)
 
 
 @pytest.mark.parametrize("kind", DTYPES)
