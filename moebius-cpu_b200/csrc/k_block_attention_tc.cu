@@ -177,7 +177,9 @@ __device__ __forceinline__ uint32_t larger(uint32_t bits, float v) {
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
-    const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+    float x, y;
+    unpair(fma2(pair(f.x, f.y), pair(-1.0f, -1.0f), pair(a, b)), x, y);
+    const __half2 r = __floats2half2_rn(x, y);
     hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&r);
 }
 
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                 tc_fence_after();
             }
             const float mc = (ref == -INFINITY ? 0.0f : ref) * c - (SPLIT ? (float)kWeightExp : 0.0f);
-            float sum[4] = {};
+            uint64_t sum[1] = {0};
 #pragma unroll
             for (int q = KEYS / 64 - 1; q >= 0; --q) {  // the last 64 keys first: they are in registers
                 if (q < KEYS / 64 - 1) {
@@ -467,9 +469,11 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float p0 = ex2(fmaf(__uint_as_float(s[g * 32 + 2 * i]), c, -mc));
-                        const float p1 = ex2(fmaf(__uint_as_float(s[g * 32 + 2 * i + 1]), c, -mc));
-                        sum[i & 1] += p0, sum[2 + (i & 1)] += p1;
+                        const int at = g * 32 + 2 * i;
+                        float p0, p1;
+                        unpair(fma2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), pair(c, c), pair(-mc, -mc)), p0, p1);
+                        p0 = ex2(p0), p1 = ex2(p1);
+                        sum[0] = add2(sum[0], pair(p0, p1));
                         if constexpr (SPLIT)
                             split2(p0, p1, hi[i], lo[i]);
                         else
@@ -479,7 +483,9 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                     if (SPLIT) tmem_st16_u32(pp + 32 + g * 16, lo);
                 }
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            float l0, l1;
+            unpair(sum[0], l0, l1);
+            l += l0 + l1;
             tmem_wait_st();
             tc_fence_before();
             arrive(kPFull + b);
