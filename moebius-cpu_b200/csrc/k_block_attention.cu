@@ -38,6 +38,7 @@ __device__ __forceinline__ void load_now(Raw8f& r, const float* p) {
 // Lanes of a key's group: the power of two that holds dim / 8.
 template <class T, int R, int U>
 __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const AttnArgs a, int lg_group) {
+    cudaGridDependencySynchronize();
     // One slot per (warp, group, row) for the join at the end: maxima, sums, outputs.
     extern __shared__ float sh[];
     __shared__ int list[kListPart];
@@ -275,8 +276,7 @@ void launch_rows(mbx_ctx* ctx, const AttnArgs& a, int64_t n) {
     MBX_REQUIRE(ctas < (int64_t(1) << 31), "block_attention: too many query rows");
     constexpr int U = (sizeof(T) == 2 ? 4 : 2) * (R == 1 ? 2 : 1);  // 128 bytes of keys and values a lane, 256 for one row
     ensure_smem_limit((const void*)attention_rows_kernel<T, R, U>, (int)smem, "attention_rows");
-    attention_rows_kernel<T, R, U><<<(unsigned)ctas, kRowWarps * 32, smem, ctx->stream>>>(a, lg_group);
-    after_launch(ctx, "attention_rows");
+    launch_after(ctx, "attention_rows", attention_rows_kernel<T, R, U>, dim3((unsigned)ctas), kRowWarps * 32, smem, a, lg_group);
 }
 
 template <class T>

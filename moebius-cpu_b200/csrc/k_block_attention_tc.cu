@@ -234,6 +234,7 @@ template <class OUT, int PANELS>
 __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2)
     attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcArgs args) {
+    cudaGridDependencySynchronize();
     constexpr bool SPLIT = is_f32<OUT>();
     constexpr bool BF16 = std::is_same<OUT, __nv_bfloat16>::value;
     constexpr int PLANES = SPLIT ? 2 : 1;
@@ -811,8 +812,8 @@ void launch_typed(mbx_ctx* ctx, const TcArgs& t, const CUtensorMap (&maps)[3]) {
     MBX_REQUIRE(ctas < (int64_t(1) << 31), "block_attention: too many query blocks");
     constexpr int smem = smem_of<PANELS, is_f32<OUT>()>();
     ensure_smem_limit((const void*)attention_tc_kernel<OUT, PANELS>, smem, "attention_tc");
-    attention_tc_kernel<OUT, PANELS><<<(unsigned)ctas, kThreads, smem, ctx->stream>>>(maps[0], maps[1], maps[2], t);
-    after_launch(ctx, "attention_tc");
+    launch_after(ctx, "attention_tc", attention_tc_kernel<OUT, PANELS>, dim3((unsigned)ctas), kThreads, smem, maps[0], maps[1],
+                 maps[2], t);
 }
 
 }  // namespace

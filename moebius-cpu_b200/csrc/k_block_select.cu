@@ -52,6 +52,7 @@ constexpr int kRing = 8;
 
 template <class T>
 __global__ void __launch_bounds__(kMeanThreads, 5) block_means_kernel(const __grid_constant__ MeanArgs args) {
+    cudaGridDependencySynchronize();
     constexpr int E = 16 / sizeof(T);  // channels of a piece
     __shared__ __align__(16) uint8_t ring[kRing * kMeanThreads * 16];
     __shared__ uint8_t keep[MBX_ATTENTION_BLOCK_Q];
@@ -324,8 +325,7 @@ template <class T>
 void launch_means(mbx_ctx* ctx, const MeanArgs& a, int64_t n) {
     const dim3 grid((unsigned)(a.side[0].blocks + a.side[1].blocks),
                     (unsigned)std::max(a.side[0].groups, a.side[1].groups), (unsigned)n);
-    block_means_kernel<T><<<grid, kMeanThreads, 0, ctx->stream>>>(a);
-    after_launch(ctx, "block_means");
+    launch_after(ctx, "block_means", block_means_kernel<T>, grid, kMeanThreads, 0, a);
 }
 
 MeanSide mean_side(const void* x, int dtype, int64_t stride, int64_t rows, int block, int blocks, int64_t width,
