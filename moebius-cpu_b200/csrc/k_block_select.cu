@@ -70,34 +70,44 @@ __global__ void __launch_bounds__(kMeanThreads, 5) block_means_kernel(const __gr
         if (threadIdx.x < MBX_ATTENTION_BLOCK_Q) keep[threadIdx.x] = m;
         count = __syncthreads_count(m != 0);
     }
-    const T* x = static_cast<const T*>(a.x) + (item * a.rows + r0) * a.x_stride + ch;
-    const uint32_t slot0 = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
+    const T* next = static_cast<const T*>(a.x) + (item * a.rows + r0 + rl) * a.x_stride + ch;  // to be requested
+    const int64_t step = lanes * a.x_stride;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16;
     const int mine = rl < lanes && ch < a.width ? (rows - rl + lanes - 1) / lanes : 0;  // rows of this thread
-    auto request = [&](int i) {  // the i-th of them
+    const bool masked = a.mask != nullptr;
+    auto request = [&](int i, int slot) {  // the i-th of them
         if (i < mine) {
-            const int r = rl + i * lanes;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot0 + i % kRing * (kMeanThreads * 16)),
-                         "l"(x + r * a.x_stride), "r"(a.mask && !keep[r] ? 0 : 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ring_at + slot * (kMeanThreads * 16)),
+                         "l"(next), "r"(masked && !keep[rl + i * lanes] ? 0 : 16)
                          : "memory");
+            next += step;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     double sum[E] = {};
 #pragma unroll
-    for (int i = 0; i < kRing; ++i) request(i);
-    for (int i = 0; i < mine; ++i) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
-        const uint4 raw = *reinterpret_cast<const uint4*>(ring + (i % kRing * kMeanThreads + threadIdx.x) * 16);
-        float v[E];
-        if constexpr (E == 8) {
-            widen8<T>(raw, v);
-        } else {
-            v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y);
-            v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
-        }
-        request(i + kRing);
+    for (int i = 0; i < kRing; ++i) request(i, i);
+    for (int i0 = 0; i0 < mine; i0 += kRing) {
 #pragma unroll
-        for (int c = 0; c < E; ++c) sum[c] += (double)v[c];
+        for (int slot = 0; slot < kRing; ++slot) {
+            if (i0 + slot >= mine) break;
+            asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+            uint4 raw;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(raw.x), "=r"(raw.y), "=r"(raw.z), "=r"(raw.w)
+                         : "r"(ring_at + slot * (kMeanThreads * 16))
+                         : "memory");
+            float v[E];
+            if constexpr (E == 8) {
+                widen8<T>(raw, v);
+            } else {
+                v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y);
+                v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
+            }
+            request(i0 + slot + kRing, slot);
+#pragma unroll
+            for (int c = 0; c < E; ++c) sum[c] += (double)v[c];
+        }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
