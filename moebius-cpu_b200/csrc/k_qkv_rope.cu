@@ -101,8 +101,12 @@ __global__ void __launch_bounds__(kWarps * 32, 4) qkv_norm_rope_kernel(const __g
     Raw raw{};
     const int h_first = part * a.per_warp + g;
     const TIn* x = x0 + tl * a.x_stride + h_first * a.dim + li * 8;
+    // A lane loads what x is at only for a head and a token that exist: a step may hold more heads than a token has.
+    auto fetch = [&](int h, int t) {
+        if (holds && h < rows && t < count) raw = load_raw8(x);
+    };
     // The first step's values are on their way while the block computes its table, the next step's while it works on one.
-    if (holds && tl < count && h_first < rows) raw = load_raw8(x);
+    fetch(h_first, tl);
 
     // A thread keeps one pair and goes through the tokens (more threads than pairs share them).
     if (a.pairs > 0) {
@@ -141,7 +145,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) qkv_norm_rope_kernel(const __g
     if (HALVES) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int pos = g * a.dim + partner[ch + i];
+            const int pos = (holds ? g : 0) * a.dim + partner[ch + i];
             pa[i] = warp * 32 * 9 + pos + (pos >> 3);
         }
     }
@@ -160,10 +164,10 @@ __global__ void __launch_bounds__(kWarps * 32, 4) qkv_norm_rope_kernel(const __g
             widen8<TIn>(raw, y);
             if (h0 + step < rows) {
                 x += step * a.dim;
-                if (holds && h + step < rows) raw = load_raw8(x);
+                fetch(h + step, t);
             } else {
                 x += apart * a.x_stride - (h0 - part * a.per_warp) * a.dim;
-                if (holds && t + apart < count) raw = load_raw8(x);
+                fetch(h_first, t + apart);
             }
             const bool is_q = h < a.heads;
             if (a.norm) {

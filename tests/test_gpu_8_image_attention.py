@@ -69,6 +69,22 @@ def test_qkv_norm_rope(mbx, ctx, case):
           + ref.TINY[kind])
 
 
+# From 128 tokens an SM on, a warp takes a second token. x ends with the last token's row, and a warp's
+# step holds up to 32 / (dim / 8) heads, more than the token has in the first four.
+ROPE_LONG = [
+    (1, 18947, 1, 1, 40, (0, 20, 20), True, True, 30, "f32", "f16", 0),
+    (3, 6400, 1, 1, 64, (0, 32, 32), False, True, 100, "bf16", "bf16", 0),
+    (1, 20001, 6, 1, 24, (2, 10, 12), True, True, 30, "f32", "bf16", 0),
+    (1, 18961, 2, 0, 8, (0, 4, 4), False, False, 30, "f16", "f16", 0),
+    (1, 18955, 3, 1, 128, (16, 56, 56), True, True, 30, "f16", "f16", 0),
+    (2, 9500, 9, 3, 72, (0, 36, 36), False, True, 100, "f32", "f32", 4)]
+
+
+@pytest.mark.parametrize("case", ROPE_LONG, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_qkv_norm_rope_of_two_tokens_a_warp(mbx, ctx, case):
+    test_qkv_norm_rope(mbx, ctx, case)
+
+
 def test_qkv_norm_rope_parts(mbx, ctx):
     """q alone, k alone, no v (whose part of the row does not exist then), no positions, no gamma."""
     rng = np.random.default_rng(3)
