@@ -51,9 +51,10 @@ __all__ = ["Context", "DeviceTensor", "Param", "MbxError", "abi", "group_norm", 
 EPILOGUES = {"none": abi.EPILOGUE_NONE, "relu": abi.EPILOGUE_RELU, "glu_silu": abi.EPILOGUE_GLU_SILU}
 PAIRINGS = {"adjacent": abi.ROPE_ADJACENT, "halves": abi.ROPE_HALVES}
 
+_F32, _I32, _U8 = np.dtype(np.float32), np.dtype(np.int32), np.dtype(np.uint8)
 #: NumPy has no bfloat16: its sixteen bits as a one-field type.
 bfloat16 = np.dtype([("bfloat16", "<u2")])
-_STORAGE = {np.dtype(np.float32): abi.DTYPE_F32, np.dtype(np.float16): abi.DTYPE_F16, bfloat16: abi.DTYPE_BF16}
+_STORAGE = {_F32: abi.DTYPE_F32, np.dtype(np.float16): abi.DTYPE_F16, bfloat16: abi.DTYPE_BF16}
 
 
 class Context:
@@ -216,6 +217,13 @@ def _vp(t: Optional[DeviceTensor]) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.ptr) if t is not None else ctypes.c_void_p(0)
 
 
+def _f32(*tensors: Optional[DeviceTensor]) -> None:
+    """The dense operators read and write float32: a buffer of a narrower type would be run past its end."""
+    for t in tensors:
+        if t is not None and t.dtype != _F32:
+            raise ValueError(f"expected float32, not {t.dtype}")
+
+
 def _nhwc(x: DeviceTensor):
     if len(x.shape) != 4:
         raise ValueError("expected an NHWC tensor")
@@ -223,11 +231,13 @@ def _nhwc(x: DeviceTensor):
 
 
 def silu_inplace(x: DeviceTensor) -> DeviceTensor:
+    _f32(x)
     check(lib().mbx_silu_inplace(x.ctx.handle, x.vp, x.size))
     return x
 
 
 def add_inplace(a: DeviceTensor, b: DeviceTensor) -> DeviceTensor:
+    _f32(a, b)
     if a.size != b.size:
         raise ValueError("add length mismatch")
     check(lib().mbx_add_inplace(a.ctx.handle, a.vp, b.vp, a.size))
@@ -236,6 +246,7 @@ def add_inplace(a: DeviceTensor, b: DeviceTensor) -> DeviceTensor:
 
 def bias_temb_add(x: DeviceTensor, bias: Optional[DeviceTensor] = None, temb: Optional[DeviceTensor] = None,
                   out: Optional[DeviceTensor] = None) -> DeviceTensor:
+    _f32(x, bias, temb, out)
     n, c = x.shape[0], x.shape[-1]
     out = out or x.ctx.empty(x.shape)
     check(lib().mbx_bias_temb_add(x.ctx.handle, x.vp, n, x.size // (n * c), c, _vp(bias), _vp(temb), out.vp))
@@ -243,6 +254,7 @@ def bias_temb_add(x: DeviceTensor, bias: Optional[DeviceTensor] = None, temb: Op
 
 
 def concat_channels(a: DeviceTensor, b: DeviceTensor, out: Optional[DeviceTensor] = None) -> DeviceTensor:
+    _f32(a, b, out)
     if a.shape[:-1] != b.shape[:-1]:
         raise ValueError("concat_channels: spatial shapes differ")
     ca, cb = a.shape[-1], b.shape[-1]
@@ -253,6 +265,7 @@ def concat_channels(a: DeviceTensor, b: DeviceTensor, out: Optional[DeviceTensor
 
 def group_norm_affine(x: DeviceTensor, groups: int, eps: float, gamma: DeviceTensor, beta: DeviceTensor,
                       add: Optional[DeviceTensor] = None):
+    _f32(x, gamma, beta, add)
     n, h, w, c = _nhwc(x)
     scale, shift = x.ctx.empty((n, c)), x.ctx.empty((n, c))
     check(lib().mbx_group_norm_affine(x.ctx.handle, x.vp, n, h, w, c, groups, eps, gamma.vp, beta.vp, _vp(add),
@@ -262,6 +275,7 @@ def group_norm_affine(x: DeviceTensor, groups: int, eps: float, gamma: DeviceTen
 
 def group_norm_apply(x: DeviceTensor, scale: DeviceTensor, shift: DeviceTensor, silu: bool = False,
                      residual: Optional[DeviceTensor] = None, out: Optional[DeviceTensor] = None) -> DeviceTensor:
+    _f32(x, scale, shift, residual, out)
     n, c = x.shape[0], x.shape[-1]
     out = out or x.ctx.empty(x.shape)
     check(lib().mbx_group_norm_apply(x.ctx.handle, x.vp, n, x.size // (n * c), c, scale.vp, shift.vp, int(silu),
@@ -272,6 +286,7 @@ def group_norm_apply(x: DeviceTensor, scale: DeviceTensor, shift: DeviceTensor, 
 def group_norm(x: DeviceTensor, groups: int, eps: float, gamma: DeviceTensor, beta: DeviceTensor,
                add: Optional[DeviceTensor] = None, silu: bool = False,
                out: Optional[DeviceTensor] = None) -> DeviceTensor:
+    _f32(x, gamma, beta, add, out)
     n, h, w, c = _nhwc(x)
     out = out or x.ctx.empty(x.shape)
     check(lib().mbx_group_norm_forward(x.ctx.handle, x.vp, n, h, w, c, groups, eps, gamma.vp, beta.vp, _vp(add),
@@ -281,6 +296,7 @@ def group_norm(x: DeviceTensor, groups: int, eps: float, gamma: DeviceTensor, be
 
 def layer_norm(x: DeviceTensor, gamma: DeviceTensor, beta: DeviceTensor, eps: float,
                out: Optional[DeviceTensor] = None) -> DeviceTensor:
+    _f32(x, gamma, beta, out)
     c = x.shape[-1]
     out = out or x.ctx.empty(x.shape)
     check(lib().mbx_layer_norm(x.ctx.handle, x.vp, x.size // c, c, gamma.vp, beta.vp, eps, out.vp))
@@ -290,6 +306,7 @@ def layer_norm(x: DeviceTensor, gamma: DeviceTensor, beta: DeviceTensor, eps: fl
 def depthwise3x3(x: DeviceTensor, weight: DeviceTensor, bias: DeviceTensor, epilogue: str = "none",
                  out: Optional[DeviceTensor] = None, prologue=None) -> DeviceTensor:
     """prologue = (scale [n, c], shift [n, c], silu): the input is read as [SiLU](x*scale + shift)."""
+    _f32(x, weight, bias, out, *(prologue or ())[:2])
     n, h, w, c = _nhwc(x)
     ep = EPILOGUES[epilogue]
     out = out or x.ctx.empty((n, h, w, c // 2 if ep == abi.EPILOGUE_GLU_SILU else c))
@@ -304,6 +321,7 @@ def depthwise3x3(x: DeviceTensor, weight: DeviceTensor, bias: DeviceTensor, epil
 
 def conv1x1(x: DeviceTensor, weight: Param, bias: Optional[DeviceTensor] = None,
             residual: Optional[DeviceTensor] = None, out: Optional[DeviceTensor] = None) -> DeviceTensor:
+    _f32(x, bias, residual, out)
     n, h, w, c = _nhwc(x)
     out = out or x.ctx.empty((n, h, w, weight.c_out))
     check(lib().mbx_conv1x1(x.ctx.handle, x.vp, n, h, w, c, weight.handle, _vp(bias), _vp(residual), out.vp))
@@ -321,6 +339,7 @@ def conv3x3(x: DeviceTensor, weight: Param, bias: Optional[DeviceTensor] = None,
             pad=(1, 1, 1, 1), upsample2x: bool = False, prologue=None, residual: Optional[DeviceTensor] = None,
             out: Optional[DeviceTensor] = None) -> DeviceTensor:
     """prologue = (scale [n, c_in], shift [n, c_in], silu) device tensors, or None."""
+    _f32(x, bias, residual, out, *(prologue or ())[:2])
     n, h, w, c = _nhwc(x)
     ho, wo = conv3x3_output_hw(h, w, stride, pad, upsample2x)
     out = out or x.ctx.empty((n, ho, wo, weight.c_out))
@@ -339,6 +358,7 @@ def conv_group_norm_affine(x: DeviceTensor, weight: Param, groups: int, eps: flo
     """A 1x1 or 3x3 conv (by the weight's taps) plus the GroupNorm affine of its output from statistics
     gathered in the conv's epilogue (mbx_conv_group_norm_affine): returns (out, scale [n, c_out],
     shift [n, c_out])."""
+    _f32(x, gamma, beta, bias, add, residual, out, *(prologue or ())[:2])
     n, h, w, c = _nhwc(x)
     ho, wo = conv3x3_output_hw(h, w, stride, pad, upsample2x) if weight.taps == 9 else (h, w)
     out = out or x.ctx.empty((n, ho, wo, weight.c_out))
@@ -354,6 +374,7 @@ def conv_group_norm_affine(x: DeviceTensor, weight: Param, groups: int, eps: flo
 def matmul(a: DeviceTensor, b: DeviceTensor, c: Optional[DeviceTensor] = None,
            accumulate: bool = False) -> DeviceTensor:
     """c (+)= a @ b for dense row-major 2-D device tensors."""
+    _f32(a, b, c)
     m, k = a.shape
     k2, n = b.shape
     if k != k2:
@@ -365,7 +386,6 @@ def matmul(a: DeviceTensor, b: DeviceTensor, c: Optional[DeviceTensor] = None,
 
 # These calls are made per layer and step, some of them shorter than a microsecond of Python: addresses go to ctypes as
 # plain integers and types are compared as the dtype objects they are.
-_F32, _I32, _U8 = np.dtype(np.float32), np.dtype(np.int32), np.dtype(np.uint8)
 _Int64x3 = ctypes.c_int64 * 3
 
 

@@ -152,6 +152,35 @@ def test_python_front_end_refuses_mismatched_tensors(mbx):
                           out=(t((1, 4, 2, 16)), t((1, 4, 1, 16)), t((1, 4, 1, 16))))
 
 
+def test_float32_operators_refuse_the_16_bit_tensors(mbx):
+    """The other operators work on float32: half-precision heads handed to one would be read past their end."""
+    def t(shape, dtype=np.float32):
+        return mbx.DeviceTensor.wrap(None, A, shape, dtype=dtype)
+
+    class Weight:  # of a convolution; the checks come before its handle
+        c_out, taps, handle = 16, 1, None
+    image, vector, rows = (1, 4, 4, 16), (16,), (16, 16)
+    calls = {
+        "silu_inplace": [image], "add_inplace": [image, image], "bias_temb_add": [image, vector],
+        "concat_channels": [image, image], "group_norm_apply": [image, (1, 16), (1, 16)],
+        "layer_norm": [image, vector, vector], "depthwise3x3": [image, (16, 9), vector], "matmul": [rows, rows]}
+    for dtype in (np.float16, mbx.bfloat16):
+        for name, shapes in calls.items():
+            for bad in range(len(shapes)):
+                args = [t(s, dtype if i == bad else np.float32) for i, s in enumerate(shapes)]
+                with pytest.raises(ValueError, match="float32"):
+                    getattr(mbx, name)(*args, *([1e-5] if name == "layer_norm" else []))
+        x, v, f = t(image, dtype), t(vector, dtype), t(vector)
+        for call in (lambda: mbx.conv1x1(x, Weight), lambda: mbx.conv1x1(t(image), Weight, residual=x),
+                     lambda: mbx.conv1x1(t(image), Weight, out=x), lambda: mbx.conv3x3(x, Weight),
+                     lambda: mbx.conv3x3(t(image), Weight, bias=v),
+                     lambda: mbx.conv3x3(t(image), Weight, prologue=(f, v, True)),
+                     lambda: mbx.group_norm(x, 4, 1e-5, f, f), lambda: mbx.group_norm_affine(t(image), 4, 1e-5, v, f),
+                     lambda: mbx.conv_group_norm_affine(x, Weight, 4, 1e-5, f, f)):
+            with pytest.raises(ValueError, match="float32"):
+                call()
+
+
 def test_oracle_rotation_is_a_rotation():
     """Pairs keep their length, and a shift of all positions leaves products of equal shifts alone."""
     rng = np.random.default_rng(0)
