@@ -144,7 +144,7 @@ class DeviceTensor:
         self.ctx = ctx
         self.shape = tuple(shape)
         self.dtype = np.dtype(dtype)
-        self.size = math.prod(self.shape)
+        self.size = math.prod(int(s) for s in self.shape)
         self.nbytes = self.dtype.itemsize * self.size
         self.owned = ptr is None
         self.ptr = ctx.alloc(self.nbytes) if ptr is None else int(ptr)

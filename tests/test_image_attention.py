@@ -152,6 +152,13 @@ def test_python_front_end_refuses_mismatched_tensors(mbx):
                           out=(t((1, 4, 2, 16)), t((1, 4, 1, 16)), t((1, 4, 1, 16))))
 
 
+def test_tensor_size_is_a_plain_integer(mbx):
+    """A shape of NumPy's narrow integers must not wrap around (or warn) on its way to a size in bytes."""
+    t = mbx.DeviceTensor(None, (np.int32(1 << 16), np.int32(1 << 16), np.uint8(3)), ptr=A)
+    assert t.size == 3 << 32 and t.nbytes == 12 << 32 and type(t.size) is int and type(t.nbytes) is int
+    assert mbx.DeviceTensor(None, (), ptr=A).size == 1 and mbx.DeviceTensor(None, (0, 5), ptr=A).size == 0
+
+
 def test_float32_operators_refuse_the_16_bit_tensors(mbx):
     """The other operators work on float32: half-precision heads handed to one would be read past their end."""
     def t(shape, dtype=np.float32):
