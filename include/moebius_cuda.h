@@ -105,7 +105,10 @@ int32_t mbx_selftest_wait_timeout(mbx_ctx *ctx, int64_t cycles);
 
 /* ---------------------------------------------------------------- memory
  * A stream-ordered best-fit caching pool: the device analogue of the
- * reference's Scratch (src/engine/mod.rs:25-117, best_fit :104-117). */
+ * reference's Scratch (src/engine/mod.rs:25-117, best_fit :104-117). A block that
+ * mbx_free hands back goes to later work of the stream that the context has then;
+ * to that of other streams only after mbx_ctx_synchronize on it. Work that a
+ * captured graph does with a block is not seen: keep such blocks while the graph lives. */
 int32_t mbx_alloc(mbx_ctx *ctx, size_t bytes, void **out);
 int32_t mbx_free(mbx_ctx *ctx, void *ptr);
 /* Frees cached blocks smaller than min_bytes (Scratch::release_below, src/engine/mod.rs:94-97). */

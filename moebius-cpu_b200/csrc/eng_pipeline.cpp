@@ -690,6 +690,7 @@ int32_t mbx_engine_set_stream(mbx_engine* engine, void* stream) {
         // Graphs were captured on the old stream; they replay on any stream, but their
         // private pools assume stream order, so the old stream is drained first.
         check_cuda(cudaStreamSynchronize(engine->ctx->stream), "cudaStreamSynchronize");
+        engine->ctx->pool->settle(engine->ctx->stream);
         ck(mbx_ctx_set_stream(engine->ctx, stream));
     });
 }

@@ -19,7 +19,7 @@ Tensor::Tensor(mbx_ctx* ctx, int64_t n_, int64_t h_, int64_t w_, int64_t c_)
     : n(n_), h(h_), w(w_), c(c_), ctx_(ctx), pool_(ctx->pool) {
     MBX_REQUIRE(n >= 0 && h >= 0 && w >= 0 && c >= 0, "negative tensor shape");
     const size_t bytes = size_t(size()) * sizeof(float);
-    p_ = bytes ? static_cast<float*>(pool_->alloc(bytes)) : nullptr;
+    p_ = bytes ? static_cast<float*>(pool_->alloc(bytes, ctx->stream)) : nullptr;
 }
 
 Tensor Tensor::view(mbx_ctx* ctx, float* p, int64_t n, int64_t h, int64_t w, int64_t c) {
@@ -37,7 +37,7 @@ Tensor Tensor::view(mbx_ctx* ctx, float* p, int64_t n, int64_t h, int64_t w, int
 Tensor::~Tensor() {
     if (p_ && pool_) {
         try {
-            pool_->free(p_);
+            pool_->free(p_, ctx_->stream);
         } catch (...) {
         }
     }
@@ -47,7 +47,7 @@ Tensor& Tensor::operator=(Tensor&& o) noexcept {
     if (this != &o) {
         if (p_ && pool_) {
             try {
-                pool_->free(p_);
+                pool_->free(p_, ctx_->stream);
             } catch (...) {
             }
         }

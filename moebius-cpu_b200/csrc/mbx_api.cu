@@ -135,19 +135,19 @@ inline float tf32_rn(float v) {
 namespace mbx {
 
 Pool::~Pool() {
-    for (auto& kv : free_) cudaFree(kv.second);
+    for (auto& kv : free_) cudaFree(kv.second.p);
     for (auto& kv : used_) cudaFree(kv.first);
 }
 
-void* Pool::alloc(size_t bytes) {
+void* Pool::alloc(size_t bytes, cudaStream_t stream) {
     std::lock_guard<std::mutex> lock(mu_);
     if (bytes == 0) bytes = 256;
     bytes = (bytes + 511) & ~size_t(511);
     // Best fit (Scratch::tensor_for, src/engine/mod.rs:61-66 / best_fit :104-117):
     // the smallest cached block that holds `bytes`, unless it wastes more than half.
-    auto it = free_.lower_bound(bytes);
-    if (it != free_.end() && it->first <= 2 * bytes + (size_t(1) << 20)) {
-        void* p = it->second;
+    for (auto it = free_.lower_bound(bytes); it != free_.end() && it->first <= 2 * bytes + (size_t(1) << 20); ++it) {
+        if (!it->second.settled && it->second.stream != stream) continue;
+        void* p = it->second.p;
         size_t sz = it->first;
         free_.erase(it);
         cached_ -= sz;
@@ -160,7 +160,7 @@ void* Pool::alloc(size_t bytes) {
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         // Give cached memory back and retry once.
-        for (auto& kv : free_) cudaFree(kv.second);
+        for (auto& kv : free_) cudaFree(kv.second.p);
         free_.clear();
         cached_ = 0;
         e = cudaMalloc(&p, bytes);
@@ -174,22 +174,27 @@ void* Pool::alloc(size_t bytes) {
     return p;
 }
 
-void Pool::free(void* p) {
+void Pool::free(void* p, cudaStream_t stream) {
     std::lock_guard<std::mutex> lock(mu_);
     auto it = used_.find(p);
     if (it == used_.end()) fail(MBX_ERR_INVALID_ARGUMENT, "mbx_free: pointer not from this context's pool");
     // Most recently freed first among equal sizes (still warm in L2).
-    free_.emplace_hint(free_.lower_bound(it->second), it->second, p);
+    free_.emplace_hint(free_.lower_bound(it->second), it->second, Cached{p, stream, false});
     cached_ += it->second;
     in_use_ -= it->second;
     used_.erase(it);
+}
+
+void Pool::settle(cudaStream_t stream) {
+    std::lock_guard<std::mutex> lock(mu_);
+    for (auto& kv : free_) kv.second.settled |= kv.second.stream == stream;
 }
 
 void Pool::release_below(size_t min_bytes) {
     std::lock_guard<std::mutex> lock(mu_);
     for (auto it = free_.begin(); it != free_.end();) {
         if (it->first < min_bytes) {
-            cudaFree(it->second);
+            cudaFree(it->second.p);
             cached_ -= it->first;
             it = free_.erase(it);
         } else {
@@ -286,6 +291,7 @@ int32_t mbx_ctx_synchronize(mbx_ctx* ctx) {
         require_ctx(ctx);
         use_device(ctx);
         check_cuda(cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
+        ctx->pool->settle(ctx->stream);
         int rec[4];
         check_cuda(cudaMemcpy(rec, ctx->dev_err, sizeof(rec), cudaMemcpyDeviceToHost), "read device error record");
         if (rec[0] != mbx::kErrNone) {
@@ -310,14 +316,14 @@ int32_t mbx_alloc(mbx_ctx* ctx, size_t bytes, void** out) {
         require_ctx(ctx);
         require_ptr(out, "out");
         use_device(ctx);
-        *out = ctx->pool->alloc(bytes);
+        *out = ctx->pool->alloc(bytes, ctx->stream);
     });
 }
 
 int32_t mbx_free(mbx_ctx* ctx, void* ptr) {
     return guard([&] {
         require_ctx(ctx);
-        if (ptr) ctx->pool->free(ptr);
+        if (ptr) ctx->pool->free(ptr, ctx->stream);
     });
 }
 

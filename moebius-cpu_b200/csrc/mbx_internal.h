@@ -48,15 +48,23 @@ class Pool {
 public:
     explicit Pool(int device) : device_(device) {}
     ~Pool();
-    void* alloc(size_t bytes);
-    void free(void* p);
+    // `stream`: the one that the block's next, or last, work is on. A block that work of another stream may still read or
+    // write is not handed out.
+    void* alloc(size_t bytes, cudaStream_t stream);
+    void free(void* p, cudaStream_t stream);
+    void settle(cudaStream_t stream);  // that stream has been waited for
     void release_below(size_t min_bytes);
     size_t cached_bytes() const { return cached_; }
     size_t in_use_bytes() const { return in_use_; }
 
 private:
     int device_;
-    std::multimap<size_t, void*> free_;        // size -> block
+    struct Cached {
+        void* p;
+        cudaStream_t stream;  // of its last work
+        bool settled;         // that work is over: any stream may have it
+    };
+    std::multimap<size_t, Cached> free_;       // by size
     std::unordered_map<void*, size_t> used_;   // block -> size
     size_t cached_ = 0, in_use_ = 0;
     mutable std::mutex mu_;
@@ -285,7 +293,7 @@ struct PoolBuf {
     mbx_ctx* ctx = nullptr;
     void* p = nullptr;
     PoolBuf() = default;
-    PoolBuf(mbx_ctx* c, size_t bytes) : ctx(c), p(c->pool->alloc(bytes)) {}
+    PoolBuf(mbx_ctx* c, size_t bytes) : ctx(c), p(c->pool->alloc(bytes, c->stream)) {}
     PoolBuf(const PoolBuf&) = delete;
     PoolBuf& operator=(const PoolBuf&) = delete;
     PoolBuf(PoolBuf&& o) noexcept : ctx(o.ctx), p(o.p) { o.p = nullptr; }
@@ -302,7 +310,7 @@ struct PoolBuf {
     void release() {
         if (p && ctx) {
             try {
-                ctx->pool->free(p);
+                ctx->pool->free(p, ctx->stream);
             } catch (...) {
             }
         }

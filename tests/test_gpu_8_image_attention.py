@@ -462,3 +462,27 @@ def test_two_captured_calls_at_once(mbx, kind, nq):
             want, tol = ref.attention(*wide, index, 32, None, 0.125, kind)
             close(t["out"].numpy(), want, tol)
         del graphs
+
+
+def test_pool_keeps_streams_apart(mbx):
+    """A block freed on one stream may still be in use there: another stream gets it only after a synchronize."""
+    legacy = 1  # the legacy default stream's handle
+    with mbx.Context(0) as ctx:
+        def block():
+            t = ctx.empty((1 << 20,))
+            t.free_at = t.ptr
+            return t
+        first = block()
+        first.free()
+        ctx.set_stream(legacy)
+        second = block()
+        assert second.ptr != first.free_at
+        second.free()
+        ctx.set_stream(None)
+        again = block()
+        assert again.ptr == first.free_at  # its own stream's order is enough
+        again.free()
+        ctx.synchronize()
+        ctx.set_stream(legacy)
+        both = [block(), block()]
+        assert {t.ptr for t in both} == {first.free_at, second.free_at}
