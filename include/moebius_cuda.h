@@ -90,6 +90,8 @@ void mbx_ctx_destroy(mbx_ctx *ctx);
 /* Use `stream` (a cudaStream_t) for all later calls; NULL restores the context's own stream. */
 int32_t mbx_ctx_set_stream(mbx_ctx *ctx, void *stream);
 void *mbx_ctx_stream(mbx_ctx *ctx);
+/* *capturing = 1 while the stream records a CUDA graph, else 0. */
+int32_t mbx_ctx_is_capturing(mbx_ctx *ctx, int32_t *capturing);
 /* Waits for the stream, then reports CUDA errors and device-side wait timeouts. */
 int32_t mbx_ctx_synchronize(mbx_ctx *ctx);
 /* Number of this library's kernel launches on this context so far. */

@@ -88,6 +88,13 @@ class Context:
         return lib().mbx_ctx_stream(self.handle) or 0
 
     @property
+    def capturing(self) -> bool:
+        """Whether the stream is recording a CUDA graph."""
+        flag = ctypes.c_int32()
+        check(lib().mbx_ctx_is_capturing(self.handle, ctypes.byref(flag)))
+        return flag.value != 0
+
+    @property
     def launch_count(self) -> int:
         return int(lib().mbx_ctx_launch_count(self.handle))
 
@@ -456,8 +463,16 @@ def _scratch(ctx: Context, nbytes: int) -> DeviceTensor:
     return ctx.empty((nbytes,), np.uint8)
 
 
+def _own_scratch(ctx: Context, size, *args) -> DeviceTensor:
+    """Scratch of one call, which goes back to the pool when the call returns. A captured call's kernels would use it at
+    every replay, beside whoever has the block then."""
+    if ctx.capturing:
+        raise ValueError("a captured call needs a workspace that lives as long as its graph")
+    return size(*args)
+
+
 def block_select_workspace(q: DeviceTensor, k: DeviceTensor, block_k: int = 64) -> DeviceTensor:
-    """Scratch for block_select calls of these shapes, one at a time."""
+    """Scratch for block_select calls of these shapes, one at a time; a captured call needs one of its own."""
     need = ctypes.c_size_t()
     check(lib().mbx_block_select_workspace(*_heads(q, k), block_k, ctypes.byref(need)))
     return _scratch(q.ctx, need.value)
@@ -474,7 +489,7 @@ def block_select(q: DeviceTensor, k: DeviceTensor, topk: int, block_k: int = 64,
     out = out or q.ctx.empty(shape, np.int32)
     _fits(out, shape, _I32, "out")
     mask_at = _at(key_mask, (n, nk), _U8, "key_mask")
-    workspace = workspace or block_select_workspace(q, k, block_k)
+    workspace = workspace or _own_scratch(q.ctx, block_select_workspace, q, k, block_k)
     check(lib().mbx_block_select(q.ctx.handle, q.ptr, heads * dim if q_stride is None else q_stride, k.ptr,
                                  kv_heads * dim if k_stride is None else k_stride, _storage(q), n, nq, nk, heads,
                                  kv_heads, dim, block_k, mask_at, topk, out.ptr, workspace.ptr, workspace.nbytes))
@@ -483,7 +498,7 @@ def block_select(q: DeviceTensor, k: DeviceTensor, topk: int, block_k: int = 64,
 
 def block_attention_workspace(q: DeviceTensor, k: DeviceTensor, index: DeviceTensor,
                               block_k: int = 64) -> DeviceTensor:
-    """Scratch for block_attention calls of these shapes, one at a time."""
+    """Scratch for block_attention calls of these shapes, one at a time; a captured call needs one of its own."""
     need = ctypes.c_size_t()
     check(lib().mbx_block_attention_workspace(_storage(q), *_heads(q, k), block_k, index.shape[-1],
                                               ctypes.byref(need)))
@@ -503,7 +518,7 @@ def block_attention(q: DeviceTensor, k: DeviceTensor, v: DeviceTensor, index: De
     mask_at = _at(key_mask, (n, nk), _U8, "key_mask")
     out = out or q.ctx.empty(q.shape, q.dtype)
     _fits(out, q.shape, q.dtype, "out")
-    workspace = workspace or block_attention_workspace(q, k, index, block_k)
+    workspace = workspace or _own_scratch(q.ctx, block_attention_workspace, q, k, index, block_k)
     kv_row = kv_heads * dim
     check(lib().mbx_block_attention(q.ctx.handle, q.ptr, heads * dim if q_stride is None else q_stride, k.ptr,
                                     kv_row if k_stride is None else k_stride, v.ptr,

@@ -86,6 +86,7 @@ SIGNATURES = {
     "mbx_ctx_destroy": (None, [_vp]),
     "mbx_ctx_set_stream": (_i32, [_vp, _vp]),
     "mbx_ctx_stream": (_vp, [_vp]),
+    "mbx_ctx_is_capturing": (_i32, [_vp, ctypes.POINTER(_i32)]),
     "mbx_ctx_synchronize": (_i32, [_vp]),
     "mbx_ctx_launch_count": (_u64, [_vp]),
     "mbx_selftest_wait_timeout": (_i32, [_vp, _i64]),

@@ -284,6 +284,17 @@ int32_t mbx_ctx_set_stream(mbx_ctx* ctx, void* stream) {
 
 void* mbx_ctx_stream(mbx_ctx* ctx) { return ctx ? (void*)ctx->stream : nullptr; }
 
+int32_t mbx_ctx_is_capturing(mbx_ctx* ctx, int32_t* capturing) {
+    return guard([&] {
+        require_ctx(ctx);
+        require_ptr(capturing, "capturing");
+        use_device(ctx);
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        check_cuda(cudaStreamIsCapturing(ctx->stream, &status), "cudaStreamIsCapturing");
+        *capturing = status != cudaStreamCaptureStatusNone;
+    });
+}
+
 uint64_t mbx_ctx_launch_count(const mbx_ctx* ctx) { return ctx ? ctx->launches : 0; }
 
 int32_t mbx_ctx_synchronize(mbx_ctx* ctx) {

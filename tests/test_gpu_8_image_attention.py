@@ -486,3 +486,25 @@ def test_pool_keeps_streams_apart(mbx):
         ctx.set_stream(legacy)
         both = [block(), block()]
         assert {t.ptr for t in both} == {first.free_at, second.free_at}
+
+
+@pytest.mark.skipif(importlib.util.find_spec("torch") is None, reason="captures with torch")
+def test_a_captured_call_needs_its_own_workspace(mbx):
+    import torch
+    with mbx.Context(0) as ctx:
+        q = ctx.upload(np.ones((1, 200, 2, 16)), dtype=np.float16)
+        index, out = mbx.block_select(q, q, 2), ctx.empty(q.shape, q.dtype)
+        mbx.block_attention(q, q, q, index, out=out)
+        ctx.synchronize()
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        assert not ctx.capturing
+        with torch.cuda.graph(graph, stream=stream):
+            ctx.set_stream(stream.cuda_stream)
+            assert ctx.capturing
+            with pytest.raises(ValueError, match="workspace"):
+                mbx.block_select(q, q, 2, out=index)
+            with pytest.raises(ValueError, match="workspace"):
+                mbx.block_attention(q, q, q, index, out=out)
+        ctx.set_stream(None)
+        assert not ctx.capturing
+        del graph
