@@ -339,11 +339,11 @@ int32_t mbx_block_select(mbx_ctx *ctx, const void *q, int64_t q_stride, const vo
  * index [n][heads][ceil(nq / 128)][topk] lists for the row's query block (mbx_block_select's
  * layout, from there or from the caller) and that key_mask keeps. Entries outside
  * [0, ceil(nk / block_k)) are skipped; a block listed twice counts twice. A row with no key left
- * is zero. Masked keys and values may hold anything; the others are finite. dim <= 128; q, k, v
- * and out have the same dtype. 16-bit weights are rounded to that type before the product with v.
- * float32 operands are carried as two float16 parts at one power of two for each (item, key head) of k
- * and of v, so a value is held to about 2^-22 of itself or 2^-23 of the largest unmasked one of its head,
- * whichever is more: rows of a cache that are not written yet belong under the mask, listed or not.
+ * is zero. Masked keys and values may hold anything, and so may those of blocks that no list names; the
+ * others are finite. dim <= 128; q, k, v and out have the same dtype. 16-bit weights are rounded to that type
+ * before the product with v. Many query rows of float32 are carried as two float16 parts of every value, at one
+ * power of two for each query row's head and for each 16 keys of a head of k and of v: a value is held to 2^-22
+ * of itself or 2^-39 of the largest of those, whichever is more.
  * out must not overlap an input. workspace as for mbx_block_select (the size may be 0, and
  * workspace NULL then). */
 int32_t mbx_block_attention_workspace(int32_t dtype, int64_t n, int64_t nq, int64_t nk, int64_t heads,

@@ -510,7 +510,9 @@ def block_attention(q: DeviceTensor, k: DeviceTensor, v: DeviceTensor, index: De
                     q_stride: Optional[int] = None, k_stride: Optional[int] = None, v_stride: Optional[int] = None,
                     workspace: Optional[DeviceTensor] = None, out: Optional[DeviceTensor] = None) -> DeviceTensor:
     """softmax(scale q k^T) v over the key blocks that index lists for each 128 query rows (mbx_block_attention);
-    scale is 1 / sqrt(dim) by default."""
+    scale is 1 / sqrt(dim) by default. Masked keys, and blocks that no list names, may hold anything. 16-bit weights are
+    rounded to the type before the product with v; float32 is held to 2^-22 of a value, or 2^-39 of the largest of its head
+    among the same 16 keys."""
     n, nq, nk, heads, kv_heads, dim = _heads(q, k)
     topk = index.shape[-1]
     _fits(v, k.shape, k.dtype, "v")

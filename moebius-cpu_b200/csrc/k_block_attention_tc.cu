@@ -28,14 +28,19 @@
 // maximum outgrows it by 2^8, so O, which accumulates in TMEM over the whole list, is rarely
 // rescaled.
 //
-// f32 operands: two f16 parts of every value after a power-of-two scale (k and v beforehand, by
-// head; a query row by the thread that owns it, as it begins): a value is held to 2^-23 of itself or of
-// the largest. Three products (lo·hi, hi·lo, hi·hi; lo·lo is 2^-22 of the whole), and the weights in
-// two parts after a scale of 2^7. The tensor core truncates as it adds into its f32 accumulator, so a
-// long sum there drifts by about 2^-25 a step: after every 2 tiles the softmax threads add what has been
-// gathered to a second set of TMEM columns, rounding to nearest, and the next tile begins a fresh sum. (Of
-// 1024 keys, relative to the exact result: 1.1e-6 after 4 tiles, 5.5e-7 after 2, 2.8e-7 after each; 484, 486 and
-// 493 us. A plain f32 softmax has 5.9e-7.)
+// f32 operands: two f16 parts of every value after a power-of-two scale, each 16 keys of a head of k and
+// of v with one of their own (beforehand, attention_split_kernel), each query row with its own (as its CTA
+// begins). A value is held to 2^-22 of itself or 2^-39 of the largest that it shares the scale with, whichever
+// is more, and no other block's values matter. Three products (lo·hi, hi·lo, hi·hi; lo·lo is 2^-22 of the
+// whole), and the weights in two parts after a scale of 2^7. The scales of k go into the factor of the
+// exponents, those of v into what the weights are relative to: with x = log2 of a weight and 2^e the scale of
+// its v, O gathers 2^(x − e − m) times the scaled v, m being the running maximum of x − e, while the sum of
+// weights has a maximum of its own. Both are whole numbers, so every rescaling is exact.
+// The tensor core truncates as it adds into its f32 accumulator, so a long sum there drifts by about 2^-25 a
+// step: the softmax threads add each tile's P·V to a second set of TMEM columns, rounding to nearest, and the
+// next tile begins a fresh sum. (16 x 4096 x 8 x 40 over 1024 keys, relative to the exact result: 3.0e-7 in
+// 549 us, with sums over two tiles 5.5e-7 in 543 us; a plain f32 softmax has 5.9e-7. With 80 channels 3.0e-7
+// against 5.5e-7 and plain 5.1e-7.)
 //
 // Masked keys: S becomes −inf; their V rows become zero in shared memory (16-bit) or while
 // splitting (f32), since zero times what a mask hides may be NaN.
@@ -57,18 +62,19 @@ namespace {
 constexpr int kRows = MBX_ATTENTION_BLOCK_Q;
 constexpr uint32_t kQPanel = kRows * 128;   // bytes of 64 channels of the query block
 constexpr int kThreads = 224;
-constexpr int kSegment = 2;                 // f32: tiles of one unbroken sum (128 keys)
 // Tiles whose bits of valid keys are kept: a slot is written again 8 tiles on, when Q·Kᵀ of a tile at most 4 before
 // that is complete, which was begun when the tile two before it, or a later one, had been read.
 constexpr int kMaskSlots = 8;
 constexpr float kLazy = 8.0f;   // log2 of the largest weight
 constexpr int kWeightExp = 7;   // f32 operands: weights are scaled by 2^7 before their split, up to 2^15
-constexpr int kScaleExp = 14;   // f32 operands: a scaled head's largest magnitude is in [2^14, 2^15)
-constexpr int kFixedExp = 6;    // and the exponent that most heads get, see attention_split_kernel
+constexpr int kScaleExp = 14;   // f32 operands: the largest magnitude is scaled to [2^14, 2^15)
+constexpr int kChunk = 16;      // f32 operands: keys that share a scale; every block is a multiple
+constexpr float kNone = -1e30f;  // f32 operands: the running maxima before the first key
 
 struct TcArgs {
     AttnArgs a;
-    const uint32_t* amax;  // f32 operands: bits of the largest magnitudes, k and then v, [n][kv_heads] each
+    const int32_t* exps;  // f32 operands: exponents of the scales, k and then v, [n][kv_heads][chunks] each
+    int chunks;
     int64_t n;
     int* err;
 };
@@ -160,17 +166,16 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The exponent of the power of two that scales values whose largest magnitude has these bits.
+// The exponent of the power of two that scales values whose largest magnitude has these bits; zeros ask for as little
+// room as the smallest values.
 __device__ __forceinline__ int scale_exponent(uint32_t bits) {
-    if (bits == 0) return 0;
     return min(kScaleExp + 127 - max((int)(bits >> 23), 1), 126);
 }
-// kFixedExp fits a largest magnitude in [2^-8, 2^9): scaled, it is below 2^15, and the parts' absolute error of
-// 2^-25 is 2^-31 of the values, 2^-23 of the largest.
-__device__ __forceinline__ bool fixed_fits(uint32_t bits) {
-    return bits == 0 || ((int)(bits >> 23) >= 127 - 8 && (int)(bits >> 23) < 127 + 9);
+// 2^d for a whole number d, 0 for one of -127 or less.
+__device__ __forceinline__ float pow2(float d) {
+    d = fminf(fmaxf(d, -127.0f), 127.0f);
+    return __uint_as_float((__float_as_uint(d + 12582912.0f) + 127u) << 23);  // 3 · 2^22: d in the low bits
 }
-__device__ __forceinline__ int part_exponent(uint32_t bits) { return fixed_fits(bits) ? kFixedExp : scale_exponent(bits); }
 // The larger of two magnitudes' bits, of finite values.
 __device__ __forceinline__ uint32_t larger(uint32_t bits, float v) {
     const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
@@ -265,13 +270,14 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         kSEmpty = kSFull + NS,  // and read, where P has columns of its own
         kPFull,                 // [NS] a tile's weights are written
         kOFull = kPFull + NS,   // [2] a tile's P·V is complete
-        kOEmpty = kOFull + 2,  // f32: a segment's sum is taken
+        kOEmpty = kOFull + 2,  // f32: a tile's sum is taken
         kFin,
         kBars
     };
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[kBars];
     __shared__ volatile uint32_t valid[kMaskSlots][4];
+    __shared__ __align__(16) float k_unscale[SPLIT ? kMaskSlots : 1][4], v_exp[SPLIT ? kMaskSlots : 1][4];  // of 16 keys each
     __shared__ uint32_t q_top[SPLIT ? kRows : 1];  // f32: bits of the query rows' largest magnitudes
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
@@ -344,7 +350,6 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         // A negative scale negates Q in the instruction descriptor. The least normal value in place of 0 (a scale of
         // 0, or far below what matters) keeps −inf · c = −inf.
         float c = fabsf(a.scale);
-        int ev = 0;
         if constexpr (SPLIT) {
             // Q in two parts, a row at a power of two of its own. A warp reads whole rows: a lane takes pieces of eight
             // channels, and the rows' magnitudes meet in shared memory.
@@ -387,13 +392,12 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             }
             fence_proxy_async_smem();
             arrive(kQFull);
-            const int eq = scale_exponent(q_top[threadIdx.x]);
-            const uint32_t* kv = args.amax + (int64_t)item * a.kv_heads + kh;
-            ev = part_exponent(kv[args.n * a.kv_heads]);
-            c = ldexpf(c, -(eq + part_exponent(*kv)));
+            c = ldexpf(c, -scale_exponent(q_top[threadIdx.x]));
         }
-        c = fmaxf(c, 1.17549435e-38f);
-        float ref = -INFINITY, l = 0.0f;  // what the weights are relative to, in units of S; their sum
+        if (!SPLIT) c = fmaxf(c, 1.17549435e-38f);  // f32: with the scale of k in it
+        // What the weights are relative to, in units of S, and their sum. f32: log2 of what O is relative to, and of what
+        // the sum is.
+        float ref = SPLIT ? kNone : -INFINITY, l = 0.0f, ref_l = kNone;
         // O's columns, 16 at a time, as far as there are channels.
         auto columns = [&](auto&& f) {
 #pragma unroll
@@ -420,30 +424,65 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                         if (!(w[q * 2 + (i >> 5)] >> (i & 31) & 1u)) s[i] = 0xff800000u;
                 }
             };
+            // Maxima of 16 keys each for f32 operands, whose scales differ.
             float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int q = 0; q < KEYS / 64; ++q) {
                 read(q);
 #pragma unroll
-                for (int i = 0; i < 64; i += 2) t[i >> 1 & 3] = max3(t[i >> 1 & 3], s[i], s[i + 1]);
+                for (int i = 0; i < 64; i += 2) {
+                    const int u = SPLIT ? i / kChunk : i >> 1 & 3;
+                    t[u] = max3(t[u], s[i], s[i + 1]);
+                }
             }
-            const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+            constexpr int CHUNKS = SPLIT ? 4 : 1;
+            float cs[CHUNKS];  // factor of S in the exponent
+            float top, top_o = 0.0f;
+            bool raise;
+            if constexpr (SPLIT) {
+                const float4 fk = *reinterpret_cast<const float4*>(k_unscale[slot]), e = *reinterpret_cast<const float4*>(v_exp[slot]);
+                const float fks[4] = {fk.x, fk.y, fk.z, fk.w}, es[4] = {e.x, e.y, e.z, e.w};
+                top = top_o = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    cs[u] = fmaxf(c * fks[u], 1.17549435e-38f);
+                    t[u] *= cs[u];
+                    top = fmaxf(top, t[u]), top_o = fmaxf(top_o, t[u] - es[u]);
+                }
+                raise = top_o - ref > kLazy || top - ref_l > kLazy;
+            } else {
+                cs[0] = c;
+                top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+                raise = ref == -INFINITY ? top > ref : (top - ref) * c > kLazy;
+            }
             // Raise the reference when a weight would pass 2^8.
-            const bool raise = ref == -INFINITY ? top > ref : (top - ref) * c > kLazy;
             if (__any_sync(0xffffffffu, raise)) {
                 float f = 1.0f;
-                if (raise) {
-                    f = ref == -INFINITY ? 0.0f : ex2((ref - top) * c);
-                    ref = top;
+                if constexpr (SPLIT) {
+                    if (top_o - ref > kLazy) {
+                        const float up = ceilf(top_o);
+                        f = pow2(ref - up);
+                        ref = up;
+                    }
+                    if (top - ref_l > kLazy) {
+                        const float up = ceilf(top);
+                        l *= pow2(ref_l - up);
+                        ref_l = up;
+                    }
+                } else {
+                    if (raise) {
+                        f = ref == -INFINITY ? 0.0f : ex2((ref - top) * c);
+                        ref = top;
+                    }
+                    l *= f;
                 }
-                l *= f;
                 if (j > 0) {
                     ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 22);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
                     for (int r = 0; r < (SPLIT ? 2 : 1); ++r) {
-                        if (r == 1 && j <= kSegment) continue;  // nothing has been taken yet
+                        if (r == 1 && j == 1) continue;  // nothing has been taken yet
                         columns([&](int i) {
                             uint32_t o[16];
                             tmem_ld16_wait(lanes + kColO + r * DCOLS + i, o);
@@ -459,8 +498,24 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                 if (!ok) break;
                 tc_fence_after();
             }
-            const float mc = (ref == -INFINITY ? 0.0f : ref) * c - (SPLIT ? (float)kWeightExp : 0.0f);
-            uint64_t sum[1] = {0};
+            float mc[CHUNKS];  // log2 of what a chunk's weights are relative to
+            if constexpr (SPLIT) {
+                // Where v is so small that its weights would be lost to the sum, they are kept, but below what counts for O.
+                const float4 e = *reinterpret_cast<const float4*>(v_exp[slot]);
+                const float es[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    mc[u] = fminf(ref + es[u], ceilf(fmaxf(t[u], kNone)) + 60.0f) - (float)kWeightExp;
+            } else {
+                mc[0] = (ref == -INFINITY ? 0.0f : ref) * c;
+            }
+            uint64_t sum = 0;
+            auto gather = [&](float factor) {
+                float l0, l1;
+                unpair(sum, l0, l1);
+                l = SPLIT ? fmaf(factor, l0 + l1, l) : l + (l0 + l1);
+                sum = 0;
+            };
 #pragma unroll
             for (int q = KEYS / 64 - 1; q >= 0; --q) {  // the last 64 keys first: they are in registers
                 if (q < KEYS / 64 - 1) {
@@ -473,11 +528,13 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int at = g * 32 + 2 * i;
+                        const int at = g * 32 + 2 * i, u = SPLIT ? at / kChunk : 0;
                         float p0, p1;
-                        unpair(fma2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), pair(c, c), pair(-mc, -mc)), p0, p1);
+                        unpair(fma2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), pair(cs[u], cs[u]),
+                                    pair(-mc[u], -mc[u])), p0, p1);
                         p0 = ex2(p0), p1 = ex2(p1);
-                        sum[0] = add2(sum[0], pair(p0, p1));
+                        sum = add2(sum, pair(p0, p1));
+                        if (SPLIT && (at + 2) % kChunk == 0) gather(pow2(mc[u] + (float)kWeightExp - ref_l));
                         if constexpr (SPLIT)
                             split2(p0, p1, hi[i], lo[i]);
                         else
@@ -487,20 +544,18 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                     if (SPLIT) tmem_st16_u32(pp + 32 + g * 16, lo);
                 }
             }
-            float l0, l1;
-            unpair(sum[0], l0, l1);
-            l += l0 + l1;
+            if (!SPLIT) gather(1.0f);
             tmem_wait_st();
             tc_fence_before();
             arrive(kPFull + b);
-            if (SPLIT && j > 0 && j % kSegment == 0) {
+            if (SPLIT && j > 0) {
                 ok = warp_wait(kOFull + ((j - 1) & 1), (j - 1) >> 1, 25);
                 if (!ok) break;
                 tc_fence_after();
                 columns([&](int i) {
                     uint32_t o[16];
                     tmem_ld16_wait(lanes + kColO + i, o);
-                    if (j > kSegment) {
+                    if (j > 1) {
                         uint32_t r[16];
                         tmem_ld16_wait(lanes + kColO + DCOLS + i, r);
 #pragma unroll
@@ -518,26 +573,30 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             tc_fence_after();
             const bool store = row < a.nq;
             const int64_t at = ((int64_t)item * a.nq + row) * a.heads + h;
-            // One factor for the row: 1 / l, or for a share of the list the weights' own scale taken out.
-            const float f = a.splits > 1 ? (SPLIT ? ldexpf(1.0f, -ev - kWeightExp) : 1.0f)
-                                         : (l == 0.0f ? 0.0f : (SPLIT ? ldexpf(1.0f, -ev) : 1.0f) / l);
+            // One factor for the row: 1 / l, or for a share of the list 1. f32: the weights' own scale taken out, and what O
+            // is relative to turned into what the sum is, in two steps as the power of two may leave f32's range.
+            float f = a.splits > 1 ? (SPLIT ? 1.0f / (1 << kWeightExp) : 1.0f) : (l == 0.0f ? 0.0f : 1.0f / l), f2 = 1.0f;
+            if constexpr (SPLIT) {
+                const float e = ref - ref_l, half = floorf(0.5f * e);
+                f *= pow2(half), f2 = pow2(e - half);
+            }
             float* part = a.part + (at * a.splits + split) * (a.dim + 4);
             if (a.splits > 1 && store) {
-                part[a.dim] = ref == -INFINITY ? ref : ref * c;
-                part[a.dim + 1] = SPLIT ? ldexpf(l, -kWeightExp) : l;
+                part[a.dim] = l == 0.0f ? -INFINITY : (SPLIT ? ref_l : ref * c);
+                part[a.dim + 1] = SPLIT ? l / (1 << kWeightExp) : l;
             }
             columns([&](int i) {
                 uint32_t o[16], r[16];
                 if (tiles > 0) tmem_ld16_wait(lanes + kColO + i, o);
-                if (SPLIT && tiles > kSegment) tmem_ld16_wait(lanes + kColO + DCOLS + i, r);
+                if (SPLIT && tiles > 1) tmem_ld16_wait(lanes + kColO + DCOLS + i, r);
 #pragma unroll
                 for (int g = 0; g < 16; g += 8) {
                     float y[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float v = __uint_as_float(o[g + e]);
-                        if (SPLIT && tiles > kSegment) v += __uint_as_float(r[g + e]);
-                        y[e] = l == 0.0f ? 0.0f : v * f;
+                        if (SPLIT && tiles > 1) v += __uint_as_float(r[g + e]);
+                        y[e] = l == 0.0f ? 0.0f : (SPLIT ? v * f * f2 : v * f);
                     }
                     if (!store || i + g >= a.dim) continue;
                     if (a.splits > 1)
@@ -583,8 +642,16 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
         uint8_t keep[WORDS];
         int64_t t_key[WORDS];
         bool checks = false;  // the tile's keys are looked at one by one
+        int k_exp = 0, v_scale = 0;  // f32: the scales of the next tile's 16 keys that lanes 0-3 look after
         auto look_up = [&](int j) {
             const int box0 = (j & (batch - 1)) << lg_boxes;
+            if (SPLIT && !is_v) {
+                const int key = (lane & 3) * kChunk;
+                const int64_t t = (int64_t)__shfl_sync(0xffffffffu, tokens, box0 + (key >> lg_rows)) + (key & (rows_box - 1));
+                const int32_t* exps = args.exps + ((int64_t)item * a.kv_heads + kh) * args.chunks + t / kChunk;
+                const bool in = t < a.nk;
+                k_exp = in ? exps[0] : 0, v_scale = in ? exps[args.n * a.kv_heads * args.chunks] : 0;
+            }
             checks = is_v ? cleans : mask || (short_boxes >> box0 & box_bits);
             if (!checks) return;
 #pragma unroll
@@ -617,6 +684,10 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                 if (lane == 0) {  // handed on with K, then with S
 #pragma unroll
                     for (int i = 0; i < WORDS; ++i) valid[slot][i] = w[i];
+                }
+                if (SPLIT) {
+                    if (lane < 4) k_unscale[slot][lane] = pow2((float)-k_exp), v_exp[slot][lane] = (float)v_scale;
+                    __syncwarp();
                 }
                 load(&map_k, sk + st * OP, OP, kKFull + st, kh, token, boxes, rows_box);
             }
@@ -692,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             if (ok) ok = warp_wait(kPFull + j % NS, j / NS, 33);
             if (ok) ok = warp_wait(kVFull + st, ph, 31);
             if (ok && cleans) ok = warp_wait(kVClean + st, ph, 32);
-            if (ok && SPLIT && j > 0 && j % kSegment == 0) ok = warp_wait(kOEmpty, j / kSegment - 1, 36);
+            if (ok && SPLIT && j > 0) ok = warp_wait(kOEmpty, j - 1, 36);
             if (!ok) break;
             tc_fence_after();
             if (leader) {
@@ -702,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                     const uint32_t pa = tmem + PCOL + j % NS * KEYS + (p == 0 ? 32 : 0);
 #pragma unroll
                     for (int s = 0; s < KEYS / 16; ++s) {
-                        const bool fresh = s == 0 && (SPLIT ? p == 0 && j % kSegment == 0 : j == 0);
+                        const bool fresh = s == 0 && (SPLIT ? p == 0 : j == 0);
                         mma_16_ts(tmem + kColO, pa + s * 8,
                                   va + (uint32_t)(s * 2048 >> 4), idesc_o, fresh ? 0u : 1u);
                     }
@@ -731,73 +802,67 @@ struct SplitArgs {
     const float* x[2];    // k, v
     int64_t stride[2];    // elements between rows
     __half* parts[2];     // [2][n][rows][heads][dim]
-    uint32_t* amax;       // [2][n][heads]
+    int32_t* exps;        // [2][n][heads][chunks]
     int64_t n, rows;
-    int heads, dim;
+    int heads, dim, chunks;
     const uint8_t* mask;  // rows that count
 };
 
 constexpr int kSplitRows = 64;
 constexpr int kSplitThreads = 256;
 
-// x · 2^e in two parts: 64 rows × 32 pieces of 8 channels. Rows that the mask hides become zero.
-__device__ __forceinline__ uint32_t split_rows(const SplitArgs& a, int t, int64_t item, int64_t r0, int piece, float f) {
-    const int width = a.heads * a.dim;
-    const int64_t plane = a.n * a.rows * width, r1 = min(r0 + kSplitRows, a.rows);
-    uint32_t top = 0;
-#pragma unroll 4
-    for (int64_t r = r0 + (threadIdx.x >> 5); r < r1; r += kSplitThreads / 32) {
-        const int64_t row = item * a.rows + r;
-        float v[8] = {};
-        if (!a.mask || a.mask[row]) widen8<float>(load_raw8(a.x[t] + row * a.stride[t] + piece * 8), v);
+// One pass over k and v: 16 rows of a head get the power of two that their largest finite magnitude asks for, and are
+// written as two parts. A CTA takes 64 rows of as many whole heads as 32 lanes hold, eight channels a lane; a thread
+// has eight rows in registers while shared memory joins the magnitudes. Rows that the mask hides become zero.
+__global__ void __launch_bounds__(kSplitThreads, 2) attention_split_kernel(const __grid_constant__ SplitArgs a) {
+    cudaGridDependencySynchronize();
+    constexpr int WARPS = kSplitThreads / 32, MINE = kSplitRows / WARPS, CHUNKS = kSplitRows / kChunk;
+    __shared__ uint32_t tops[CHUNKS][32];
+    const int t = blockIdx.y & 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int lanes = a.dim / 8, per = 32 / lanes, at = lane / lanes, head0 = (int)(blockIdx.y >> 1) * per;
+    const int64_t item = blockIdx.z, r0 = (int64_t)blockIdx.x * kSplitRows;
+    const bool on = at < per && head0 + at < a.heads;
+    const int ch = head0 * a.dim + lane * 8;
+    if (threadIdx.x < CHUNKS * 32) tops[warp][lane] = 0;
+    __syncthreads();
+    Raw8f raw[MINE];  // rows warp, warp + 8, …: two of each 16
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int64_t r = r0 + warp + i * WARPS, row = item * a.rows + r;
+        raw[i] = Raw8f{};
+        if (on && r < a.rows && (!a.mask || a.mask[row])) raw[i] = load_raw8(a.x[t] + row * a.stride[t] + ch);
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = c * (MINE / CHUNKS); i < (c + 1) * (MINE / CHUNKS); ++i) {
+            float v[8];
+            widen8<float>(raw[i], v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = larger(top, v[e]);
+        }
+        if (on && top) atomicMax(&tops[c][at], top);
+    }
+    __syncthreads();
+    const int64_t width = (int64_t)a.heads * a.dim, plane = a.n * a.rows * width;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int64_t r = r0 + warp + i * WARPS;
+        if (!on || r >= a.rows) continue;
+        const float f = pow2((float)scale_exponent(tops[i / (MINE / CHUNKS)][at]));
+        float v[8];
+        widen8<float>(raw[i], v);
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            top = larger(larger(top, v[2 * e]), v[2 * e + 1]);
-            split2(v[2 * e] * f, v[2 * e + 1] * f, hi[e], lo[e]);
-        }
-        uint4* out = reinterpret_cast<uint4*>(a.parts[t] + row * width + piece * 8);
+        for (int e = 0; e < 4; ++e) split2(v[2 * e] * f, v[2 * e + 1] * f, hi[e], lo[e]);
+        uint4* out = reinterpret_cast<uint4*>(a.parts[t] + (item * a.rows + r) * width + ch);
         out[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         out[plane / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    return top;
-}
-
-// One pass over k and v: their parts at the exponent that fits almost any head, and what tells whether it does, the
-// largest finite magnitude of each head. A pass for the magnitudes alone would read everything twice: 126 us
-// for 252 MB beside 97 us for the parts.
-__global__ void __launch_bounds__(kSplitThreads) attention_split_kernel(const __grid_constant__ SplitArgs a) {
-    __shared__ uint32_t tops[32];
-    const int t = blockIdx.y & 1, lane = threadIdx.x & 31, piece = (blockIdx.y >> 1) * 32 + lane;
-    const int64_t item = blockIdx.z;
-    if (threadIdx.x < 32) tops[threadIdx.x] = 0;
-    __syncthreads();
-    const bool on = piece * 8 < a.heads * a.dim;
-    uint32_t top = 0;
-    if (on) top = split_rows(a, t, item, (int64_t)blockIdx.x * kSplitRows, piece, ldexpf(1.0f, kFixedExp));
-    const int first = (blockIdx.y >> 1) * 256 / a.dim, head = piece * 8 / a.dim;  // at most 32 heads: dim >= 8
-    if (on) atomicMax(&tops[head - first], top);
-    __syncthreads();
-    if (threadIdx.x < 32 && tops[threadIdx.x])
-        atomicMax(a.amax + (t * a.n + item) * a.heads + first + threadIdx.x, tops[threadIdx.x]);
-}
-
-// The heads that the fixed exponent does not fit, once more with their own.
-__global__ void __launch_bounds__(kSplitThreads) attention_resplit_kernel(const __grid_constant__ SplitArgs a) {
-    cudaGridDependencySynchronize();
-    const int64_t total = 2 * a.n * a.heads;
-    bool none = true;
-    for (int64_t i = threadIdx.x; i < total; i += kSplitThreads) none &= fixed_fits(a.amax[i]);
-    if (__syncthreads_and(none)) return;
-    const int groups = (a.heads * a.dim / 8 + 31) / 32;
-    const int64_t tiles = (a.rows + kSplitRows - 1) / kSplitRows, all = tiles * groups * 2 * a.n;
-    for (int64_t w = blockIdx.x; w < all; w += gridDim.x) {
-        const int t = (int)(w & 1), piece = (int)(w / 2 % groups) * 32 + (threadIdx.x & 31);
-        const int64_t item = w / 2 / groups / tiles, tile = w / 2 / groups % tiles;
-        if (piece * 8 >= a.heads * a.dim) continue;
-        const uint32_t bits = a.amax[(t * a.n + item) * a.heads + piece * 8 / a.dim];
-        if (!fixed_fits(bits)) split_rows(a, t, item, tile * kSplitRows, piece, ldexpf(1.0f, scale_exponent(bits)));
-    }
+    const int chunk = (int)(r0 / kChunk) + warp, head = head0 + lane;
+    if (warp < CHUNKS && lane < per && head < a.heads && chunk < a.chunks)
+        a.exps[((t * a.n + item) * a.heads + head) * a.chunks + chunk] = scale_exponent(tops[warp][lane]);
 }
 
 // A map over [items][rows][heads][dim] 16-bit values, boxes of 64 channels × one head × box_rows rows.
@@ -822,32 +887,31 @@ void launch_typed(mbx_ctx* ctx, const TcArgs& t, const CUtensorMap (&maps)[3]) {
 }  // namespace
 
 size_t attention_split_bytes(const BlockShape& s) {
-    return align256(4 * 2 * (size_t)(s.n * s.kv_heads)) +
+    return align256(4 * 2 * (size_t)(s.n * s.kv_heads * ((s.nk + kChunk - 1) / kChunk))) +
            2 * align256(2 * 2 * (size_t)(s.n * s.nk * s.kv_heads * s.dim));
 }
 
 void launch_attention_tc(mbx_ctx* ctx, const AttnArgs& a, int dtype, int64_t n, void* split) {
-    TcArgs t{a, nullptr, n, ctx->dev_err};
+    TcArgs t{a, nullptr, 0, n, ctx->dev_err};
     CUtensorMap maps[3];
     const bool bf16 = dtype == MBX_DTYPE_BF16;
     const int rows_box = std::min(a.block_k, dtype != MBX_DTYPE_F32 && a.dim <= 64 ? keys_of<1, false>() : keys_of<2, false>());
     if (dtype == MBX_DTYPE_F32) {
         SplitArgs s{};
-        const size_t amax_bytes = 4 * 2 * (size_t)(n * a.kv_heads);
+        s.chunks = (int)((a.nk + kChunk - 1) / kChunk);
+        const size_t exps_bytes = align256(4 * 2 * (size_t)(n * a.kv_heads * s.chunks));
         const size_t part_bytes = align256(2 * 2 * (size_t)(n * a.nk * a.kv_heads * a.dim));
-        s.amax = static_cast<uint32_t*>(split);
+        s.exps = static_cast<int32_t*>(split);
         s.n = n, s.rows = a.nk, s.heads = a.kv_heads, s.dim = a.dim, s.mask = a.mask;
         s.x[0] = static_cast<const float*>(a.k), s.x[1] = static_cast<const float*>(a.v);
         s.stride[0] = a.k_stride, s.stride[1] = a.v_stride;
         for (int i = 0; i < 2; ++i)
-            s.parts[i] = reinterpret_cast<__half*>(static_cast<uint8_t*>(split) + align256(amax_bytes) + i * part_bytes);
-        check_cuda(cudaMemsetAsync(s.amax, 0, amax_bytes, ctx->stream), "cudaMemsetAsync");
+            s.parts[i] = reinterpret_cast<__half*>(static_cast<uint8_t*>(split) + exps_bytes + i * part_bytes);
+        const int per = 32 / (a.dim / 8);  // heads of a CTA
         const dim3 grid((unsigned)((a.nk + kSplitRows - 1) / kSplitRows),
-                        (unsigned)(2 * ((a.kv_heads * a.dim / 8 + 31) / 32)), (unsigned)n);
-        attention_split_kernel<<<grid, kSplitThreads, 0, ctx->stream>>>(s);
-        after_launch(ctx, "attention_split");
-        launch_after(ctx, "attention_resplit", attention_resplit_kernel, dim3((unsigned)ctx->sm_count), kSplitThreads, 0, s);
-        t.amax = s.amax;
+                        (unsigned)(2 * ((a.kv_heads + per - 1) / per)), (unsigned)n);
+        launch_after(ctx, "attention_split", attention_split_kernel, grid, kSplitThreads, 0, s);
+        t.exps = s.exps, t.chunks = s.chunks;
         for (int i = 1; i < 3; ++i)
             encode_heads(&maps[i], s.parts[i - 1], false, 2 * n, a.nk, a.kv_heads, a.dim, (int64_t)a.kv_heads * a.dim,
                          rows_box);

@@ -285,6 +285,66 @@ def test_block_attention_of_small_and_large_values(mbx, ctx, kind, size):
     close(out.numpy(), want, tol)
 
 
+def exact_weights(rng, nq, nk, heads, dim):
+    """q and k whose logits are whole numbers, exact in any summation: 0 or -200 by the key's first channel."""
+    q, k = np.zeros((1, nq, heads, dim), np.float32), np.zeros((1, nk, 1, dim), np.float32)
+    q[..., 0] = 1.0
+    return q, k, rng.standard_normal((1, nk, 1, dim)).astype(np.float32)
+
+
+def equal_weights_tolerance(v, keys):
+    """Of the mean of v over `keys`, in units of its mean magnitude (weights are exactly 1 there): a value's two parts
+    2^-22; at most 128 keys in an unbroken sum, 8 steps of 16 keys in three products each, 2^-23 a step; their joining,
+    the sum of weights and the quotient, 8 roundings of 2^-24."""
+    return (2.0 ** -22 + 24 * 2.0 ** -23 + 8 * 2.0 ** -24) * np.abs(v[0, keys, 0].astype(np.float64)).mean(0)
+
+
+@pytest.mark.parametrize("heads", [2, 148])  # lists that are split over CTAs, and whole ones
+@pytest.mark.parametrize("nq", [2, 140])
+@pytest.mark.parametrize("typical,far", [(1.0, 4.0), (1e-4, 0.1), (1e-5, 1.0), (1.0, 1e9), (1.0, 1e30), (1e-20, 1.0)])
+def test_f32_attention_does_not_depend_on_other_blocks_values(mbx, ctx, typical, far, nq, heads):
+    """Neither a row of a block that no list names nor a listed one of no weight costs the others their bits."""
+    rng = np.random.default_rng(41)
+    nk, dim = 640, 24
+    q, k, v = exact_weights(rng, nq, nk, heads, dim)
+    v *= typical
+    v[0, 37] = far      # block 0, unlisted
+    k[0, 37] = far
+    v[0, 38], k[0, 39] = np.nan, np.inf
+    v[0, 330:336] = far  # block 5, listed; no weight
+    k[0, 320:384, 0, 0] = -200.0
+    lists = [1, 2, 3, 5, 7, 8]
+    index = np.broadcast_to(np.int32(lists), (1, heads, -(-nq // 128), len(lists))).copy()
+    out = mbx.block_attention(*(up(ctx, t) for t in (q, k, v, index)), scale=1.0).numpy()
+    keys = np.concatenate([np.arange(b * 64, b * 64 + 64) for b in lists if b != 5])
+    want = v[0, keys, 0].astype(np.float64).mean(0)
+    tol = equal_weights_tolerance(v, keys) + far * np.exp(-200.0)
+    close(out, np.broadcast_to(want, out.shape), np.broadcast_to(tol, out.shape))
+
+
+@pytest.mark.parametrize("heads", [2, 148])
+def test_f32_attention_of_blocks_of_every_magnitude(mbx, ctx, heads):
+    """Each 16 keys have values of another magnitude, zero among them, and keys of another one too."""
+    rng = np.random.default_rng(43)
+    nq, nk, dim = 140, 960, 16
+    for powers in ([-120, -20, 0, 20, 120], [-140, -130, -126], [0, 0, -400]):  # -400: zero
+        q, k, v = (rng.standard_normal((1, t, h, dim)) for t, h in ((nq, heads), (nk, 1), (nk, 1)))
+        size = 2.0 ** rng.choice(powers, nk // 16).repeat(16)
+        v = (v * size[None, :, None, None]).astype(np.float32)
+        k = (k * (2.0 ** rng.integers(-12, 3, nk // 16).repeat(16))[None, :, None, None]).astype(np.float32)
+        turn = 2.0 ** 100 if powers[0] == 0 else 1.0  # magnitudes of q and k that their products do not have
+        q, k = (q / turn).astype(np.float32), (k * turn).astype(np.float32)
+        index = np.full((1, heads, 2, 30), -1, np.int32)
+        for at in np.ndindex(index.shape[:3]):
+            index[at][:25] = np.sort(rng.permutation(30)[:25])
+        out = mbx.block_attention(*(up(ctx, t) for t in (q, k, v, index)), block_k=32, scale=0.5)
+        want, tol = ref.attention(*(ref.wide(t) for t in (q, k, v)), index, 32, None, 0.5, "f32")
+        # Below 2^-126 a rounding is off by up to 2^-150: 13 shares of the list (25 blocks of 32 keys in tiles of 64), each
+        # rounded, weighted by at most one and added with a rounding, over a sum of weights of at least 1/2 (the largest
+        # share's reference is its maximum rounded up to a whole log2): 26 * 2^-150 * 2 + 2^-150 < 2^-144.
+        close(out.numpy(), want, tol + 2.0 ** -144)
+
+
 def test_block_attention_long_list_of_one_token(mbx, ctx):
     """More list entries for one CTA than it keeps in shared memory at a time."""
     rng = np.random.default_rng(31)
