@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const At
 
 // Joins the splits' partial results: a CTA per (row, head). The splits' weights are worked out once in shared memory;
 // then each warp adds every fourth split, a lane four channels, eight splits in flight.
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 256;
 
 template <class T>
 __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a) {
@@ -196,18 +196,20 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stride = a.dim + 4;
     const float* p = a.part + (int64_t)blockIdx.x * a.splits * stride;
     if (warp == 0) {
-        float m[2], l[2];
+        constexpr int MINE = kMaxSplits / 32;
+        float m[MINE], l[MINE], top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < MINE; ++i) {
             const int s = lane + 32 * i;
             m[i] = s < a.splits ? p[s * stride + a.dim] : -INFINITY;
             l[i] = s < a.splits ? p[s * stride + a.dim + 1] : 0.0f;
         }
-        float top = fmaxf(m[0], m[1]);
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) top = fmaxf(top, m[i]);
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < MINE; ++i) {
             const float w = m[i] == -INFINITY ? 0.0f : exp2f(m[i] - top);
             weight[lane + 32 * i] = w;
             sum = fmaf(w, l[i], sum);
@@ -254,11 +256,17 @@ Plan plan_of(const BlockShape& s, int64_t topk) {
                          : s.nq <= 2 && s.n * s.heads < 64;
     if (few) p.rows = s.nq == 1 ? 1 : s.nq == 2 ? 2 : 4;
     // Enough CTAs to fill the card four times over (rows) or twice (tensor cores), with equal shares of the list's blocks
-    // or tiles of 64 keys.
+    // or tiles of 64 keys, but no more than kFillSplits.
+    constexpr int64_t kFillSplits = 64;
     const int64_t tile = p.rows ? p.rows : MBX_ATTENTION_BLOCK_Q;
     const int64_t ctas = std::max<int64_t>(1, s.n * s.heads * ((s.nq + tile - 1) / tile));
     const int64_t pieces = std::max<int64_t>(1, p.rows ? topk : (topk * s.block_k + 63) / 64);
-    const int64_t want = std::min(((p.rows ? 4 : 2) * kSms + ctas - 1) / ctas, int64_t(kMaxSplits));
+    int64_t want = std::min(((p.rows ? 4 : 2) * kSms + ctas - 1) / ctas, kFillSplits);
+    // The tensor core truncates as it adds, so a 16-bit result's unbroken sum falls behind by 2^-23.2 each 16 keys (f16,
+    // equal weights over 2^21 keys: 1.4 %, in shares of 2^15 0.03 % with the rounding). Half of the result's own half step is the most it
+    // may lose: 2^15 keys for f16, 2^18 for bf16. f32 sums are broken anyway.
+    if (!p.rows && s.dtype != MBX_DTYPE_F32)
+        want = std::max(want, (pieces * 64 - 1 >> (s.dtype == MBX_DTYPE_F16 ? 15 : 18)) + 1);
     const int64_t share = (pieces + want - 1) / want;
     p.splits = (int)((pieces + share - 1) / share);
     if (p.splits > 1)

@@ -364,6 +364,24 @@ def test_block_attention_long_list_of_one_token(mbx, ctx):
     close(out.numpy()[0, 0], want, tol + ref.HALF_STEP["f16"] * (np.abs(want) + tol))
 
 
+@pytest.mark.parametrize("dim", [8, 72])
+def test_block_attention_long_list_of_many_rows(mbx, ctx, dim):
+    """Equal weights over two million keys: the tensor core truncates its sums, which must not show in the mean.
+
+    Positive values, so that truncations add up: 2048 steps of 16 keys in an unbroken sum, in two additions each that
+    lose up to 2^-23; joining, the sum of weights and the quotient 2^-16; the result's rounding."""
+    rng = np.random.default_rng(47)
+    heads, nq, nk, block_k = 150, 129, 1 << 21, 128  # 300 query blocks fill the card: lists need not be split
+    v = (0.5 + 0.5 * rng.random((1, nk, 1, dim))).astype(np.float16)
+    index = np.broadcast_to(np.arange(nk // block_k, dtype=np.int32), (1, heads, 2, nk // block_k))
+    q, d = up(ctx, np.zeros((1, nq, heads, dim), np.float16)), up(ctx, v)
+    out = mbx.block_attention(q, d, d, up(ctx, np.ascontiguousarray(index)), block_k=block_k).numpy()
+    want = np.broadcast_to(v[0, :, 0].astype(np.float64).mean(0), out.shape)
+    close(out, want, (2048 * 2.0 ** -22 + 2.0 ** -16 + 2.0 ** -11) * want)
+    ctx.synchronize()
+    ctx.release_below(1 << 62)
+
+
 @pytest.mark.parametrize("kind,nq", [("f32", 1), ("f16", 1), ("bf16", 200)])
 def test_offsets_past_32_bits(mbx, ctx, kind, nq):
     """Keys and values in rows of 1024 elements, over two million tokens on: element offsets past 2^31."""
