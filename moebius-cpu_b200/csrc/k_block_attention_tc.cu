@@ -48,7 +48,8 @@
 // 53 % busy, exponentials 54 %), 2 x 16384 x 16 x 64 f16 over 2048 keys in 414 us (664 TFLOP/s; exponentials 63 %),
 // 16 x 4096 x 8 x 40 f32 over 1024 keys in 477 us with the split (180 TFLOP/s, 540 in products).
 // Every wait is bounded; on timeout the CTA records the error, waits (bounded) for its copies and
-// MMAs in flight, frees TMEM and returns.
+// MMAs in flight, frees TMEM and returns. It looks for them when every warp has stopped: a producer may be through
+// with its part before another warp gives up.
 #include <algorithm>
 #include <type_traits>
 
@@ -237,6 +238,33 @@ constexpr bool is_f32() {
     return std::is_same<OUT, float>::value;
 }
 
+// After a timeout, when every warp has stopped: MMAs in flight finish before TMEM is freed, and copies land before the
+// CTA's memory is given up. Out of line, as the kernel needs its registers.
+struct Settle {
+    int fin, q_full, k_full, v_full;
+    bool split;
+    int stages;
+};
+__device__ __noinline__ void settle(uint32_t bars, Settle s, const int* issued, int* err) {
+    const long long deadline = clock64() + kWaitLimit;
+    const int warp = threadIdx.x >> 5;
+    auto drain = [&](int b, int phase, int site) {
+        drain_wait(bars + 8u * (uint32_t)b, (uint32_t)phase & 1u, deadline, err, site, kKAttention);
+    };
+    if (warp == 5) {
+        if (elect_one()) {  // the lane that issued them
+            mma_commit(bars + 8u * (uint32_t)s.fin);
+            drain(s.fin, 0, 34);
+        }
+        __syncwarp();
+    } else if (warp >= 4 && (threadIdx.x & 31) == 0) {
+        const int v = warp == 6, done = issued[v];
+        if (!s.split && !v && done > 0) drain(s.q_full, 0, 40);  // Q comes with tile 0, which waits for nothing
+        for (int i = max(0, done - s.stages); i < done; ++i) drain((v ? s.v_full : s.k_full) + i % s.stages, i / s.stages, 40);
+    }
+    __syncthreads();
+}
+
 // OUT: the type of the tensors; the operands' type is OUT, or f16 parts where OUT is float.
 template <class OUT, int PANELS>
 __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2)
@@ -280,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
     __shared__ __align__(16) float k_unscale[SPLIT ? kMaskSlots : 1][4], v_exp[SPLIT ? kMaskSlots : 1][4];  // of 16 keys each
     __shared__ uint32_t q_top[SPLIT ? kRows : 1];  // f32: bits of the query rows' largest magnitudes
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, issued[2];  // issued: tiles of K, of V whose copies were begun
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t sv = base, sk = sv + STAGES * OP, sq = sk + STAGES * OP;
@@ -715,14 +743,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                 if (lane == 0) mbar_arrive(bar(kVClean + st));
             }
         }
-        __syncwarp();
-        if (*abort_p && lane == 0) {  // copies in flight land before the CTA's memory is given up
-            const long long deadline = clock64() + kWaitLimit;
-            if (!SPLIT && !is_v && tiles > 0) drain_wait(bar(kQFull), 0, deadline, args.err, 40, kKAttention);
-            for (int i = std::max(0, done - STAGES); i < done; ++i)
-                drain_wait(bar((is_v ? kVFull : kKFull) + i % STAGES), (uint32_t)(i / STAGES) & 1u, deadline, args.err, 40,
-                           kKAttention);
-        }
+        if (lane == 0) issued[is_v] = done;
     } else if (tiles > 0) {
         // ---------------------------------------------------------------- MMA issuer
         // The whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues.
@@ -784,15 +805,12 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             __syncwarp();
             if (!OWN_P && j + 2 < tiles) ok = scores(j + 2);
         }
-        if (!ok && leader) {  // MMAs in flight finish before TMEM is freed
-            mma_commit(bar(kFin));
-            drain_wait(bar(kFin), 0, clock64() + kWaitLimit, args.err, 34, kKAttention);
-        }
-        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (*abort_p)  // the same for all: nobody waits any more
+        settle(smem_u32(bars), {kFin, kQFull, kKFull, kVFull, SPLIT, STAGES}, issued, args.err);
     if (warp == 5) tmem_dealloc(tmem, TMEM);
 }
 
