@@ -71,7 +71,7 @@ __device__ __forceinline__ float head_sum(float v, int L, int li, int lane0) {
             ++n;
         }
     }
-    return t;
+    return __shfl_sync(0xffffffffu, t, lane0);  // the lanes added in different orders
 }
 
 __device__ __forceinline__ void read8(float (&v)[8], const float* p) {

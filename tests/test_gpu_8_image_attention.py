@@ -110,6 +110,18 @@ def test_qkv_norm_rope_parts(mbx, ctx):
     assert [t.shape for t in empty] == [(2, 0, 1, 16)] * 3
 
 
+@pytest.mark.parametrize("dim", [24, 40, 64, 72, 80, 104, 200])
+def test_qkv_norm_rope_has_one_factor_a_head(mbx, ctx, dim):
+    """The norm's factor is the head's: every eighth channel is 1 here, so it is the factor itself."""
+    rng = np.random.default_rng(dim)
+    x = rng.standard_normal((1, 500, 3, dim)).astype(np.float32)
+    x[..., ::8] = 1.0
+    q, k, _ = mbx.qkv_norm_rope(up(ctx, x.reshape(1, 500, 3 * dim)), 1, 1, dim)
+    for got in (q.numpy(), k.numpy()):
+        factors = got[..., ::8]
+        assert (factors == factors[..., :1]).all()
+
+
 def test_qkv_norm_rope_keeps_nan_in_its_head(mbx, ctx):
     x = np.ones((1, 3, 4 * 8), np.float32)
     x[0, 1, 8] = np.nan
