@@ -295,7 +295,9 @@ int32_t mbx_scale_add(mbx_ctx *ctx, const float *x, int64_t len, float mul, floa
  * heads. A *_stride is the number of elements between two tokens, at least the
  * row's own length, so a part of a packed row serves in place; item i starts at
  * i * tokens * stride. Pointers are 16-byte aligned, rows a multiple of 16 bytes
- * apart, dim a multiple of 8. The results are deterministic. */
+ * apart, dim a multiple of 8. The results are deterministic. Limits: tokens and n * tokens of
+ * mbx_qkv_norm_rope below 2^31 - 256, strides below 2^31; for the other two n * heads at most 65535,
+ * heads at most 16384, topk at most 65536 and n * heads * ceil(nq / 128) below 2^31. */
 
 /* Splits the rows of a packed projection x [n][tokens][x_stride], each
  * [q heads | k kv_heads | v kv_heads] x dim, into q [n][tokens][heads][dim] and
@@ -326,7 +328,9 @@ int32_t mbx_qkv_norm_rope(mbx_ctx *ctx, const void *x, int32_t x_dtype, int64_t 
  * -1 where fewer blocks have an unmasked key. key_mask [n][nk] bytes, nonzero = may be
  * attended to (NULL: all); masked keys may hold anything. Means and scores are float64, so the
  * choice does not hang on the order of a sum; a score of NaN counts as the highest.
- * workspace: mbx_block_select_workspace bytes of device memory, 256-byte aligned, that no
+ * dim <= 256, nq at most 536862720.
+ * workspace (8 bytes for every pair of a query block and a key block of a head, mostly):
+ * mbx_block_select_workspace bytes of device memory, 256-byte aligned, that no
  * other call in flight uses. */
 int32_t mbx_block_select_workspace(int64_t n, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t dim,
                                    int64_t block_k, size_t *bytes);

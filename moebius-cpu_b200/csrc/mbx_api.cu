@@ -79,11 +79,19 @@ mbx::BlockShape block_shape(int32_t dtype, int64_t n, int64_t nq, int64_t nk, in
     return mbx::BlockShape{dtype, n, nq, nk, heads, kv_heads, dim, block_k};
 }
 
+// `most`: query blocks of one item and head.
+void require_query_blocks(const mbx::BlockShape& s, int64_t most) {
+    const int64_t q_blocks = (s.nq + MBX_ATTENTION_BLOCK_Q - 1) / MBX_ATTENTION_BLOCK_Q;
+    MBX_REQUIRE(q_blocks <= most && s.n * s.heads * q_blocks < (int64_t(1) << 31), "too many query blocks");
+}
+
 void require_topk(const mbx::BlockShape& s, int64_t topk) {
     MBX_REQUIRE(topk >= 0 && topk <= 65536, "topk must be in [0, 65536]");
-    const int64_t q_blocks = (s.nq + MBX_ATTENTION_BLOCK_Q - 1) / MBX_ATTENTION_BLOCK_Q;
-    MBX_REQUIRE(s.n * s.heads * q_blocks < (int64_t(1) << 31), "too many query blocks");
+    require_query_blocks(s, kMaxExtent);
 }
+
+// A grid's y extent counts 64 query blocks in block_select.
+constexpr int64_t kSelectQueryBlocks = 64 * 65535;
 
 void require_workspace(const void* p, size_t have, size_t need) {
     if (need == 0) return;
@@ -834,8 +842,9 @@ int32_t mbx_block_select_workspace(int64_t n, int64_t nq, int64_t nk, int64_t he
                                    int64_t block_k, size_t* bytes) {
     return guard([&] {
         require_ptr(bytes, "bytes");
-        *bytes = mbx::block_select_bytes(block_shape(MBX_DTYPE_F32, n, nq, nk, heads, kv_heads, dim, block_k,
-                                                     mbx::kRopeMaxDim));
+        const mbx::BlockShape s = block_shape(MBX_DTYPE_F32, n, nq, nk, heads, kv_heads, dim, block_k, mbx::kRopeMaxDim);
+        require_query_blocks(s, kSelectQueryBlocks);
+        *bytes = mbx::block_select_bytes(s);
     });
 }
 
@@ -847,6 +856,7 @@ int32_t mbx_block_select(mbx_ctx* ctx, const void* q, int64_t q_stride, const vo
         require_ctx(ctx);
         const mbx::BlockShape s = block_shape(dtype, n, nq, nk, heads, kv_heads, dim, block_k, mbx::kRopeMaxDim);
         require_topk(s, topk);
+        require_query_blocks(s, kSelectQueryBlocks);
         require_rows(q, q_stride, heads * dim, dtype, "q");
         require_rows(k, k_stride, kv_heads * dim, dtype, "k");
         if (n == 0 || nq == 0 || topk == 0) return;

@@ -114,6 +114,16 @@ def test_workspace_sizes_refuse_what_the_calls_refuse(mbx, change, text):
                                                                       "block_k")], None), "bytes")
 
 
+@pytest.mark.parametrize("change", [dict(nq=1 << 30, heads=1024, nk=1 << 30),  # a size that would wrap around
+                                    dict(nq=64 * 65535 * 128 + 1, n=1, heads=1)])
+def test_block_select_refuses_too_many_query_blocks(mbx, blank, change):
+    a, need = {**BLOCK, **change}, ctypes.c_size_t()
+    a.update(q_stride=a["heads"] * a["dim"])
+    shape = [a[s] for s in ("n", "nq", "nk", "heads", "kv_heads", "dim", "block_k")]
+    _refused(mbx, mbx.abi.lib().mbx_block_select_workspace(*shape, ctypes.byref(need)), "query blocks")
+    _refused(mbx, _select(mbx, blank, a), "query blocks")
+
+
 def test_null_context(mbx):
     _refused(mbx, _select(mbx, None, BLOCK), "context")
     _refused(mbx, _attend(mbx, None, BLOCK), "context")
