@@ -403,17 +403,23 @@ def _storage(t: DeviceTensor) -> int:
     return code
 
 
-def _fits(t: DeviceTensor, shape: tuple, dtype: np.dtype, what: str) -> None:
-    """A tensor of the caller's holds what a kernel reads or writes there."""
+def _near(t: DeviceTensor, ctx: Context, what: str) -> None:
+    if t.ctx is not ctx and t.ctx.device != ctx.device:
+        raise ValueError(f"{what} is on another device")
+
+
+def _fits(t: DeviceTensor, shape: tuple, dtype: np.dtype, what: str, ctx: Context) -> None:
+    """A tensor of the caller's holds what a kernel of ctx reads or writes there."""
+    _near(t, ctx, what)
     if t.shape != shape or (t.dtype is not dtype and t.dtype != dtype):
         raise ValueError(f"{what} must be {dtype} of shape {shape}, not {t.dtype} of {t.shape}")
 
 
-def _at(t: Optional[DeviceTensor], shape: tuple, dtype: np.dtype, what: str) -> Optional[int]:
+def _at(t: Optional[DeviceTensor], shape: tuple, dtype: np.dtype, what: str, ctx: Context) -> Optional[int]:
     """The address of a tensor that may be left out."""
     if t is None:
         return None
-    _fits(t, shape, dtype, what)
+    _fits(t, shape, dtype, what, ctx)
     return t.ptr
 
 
@@ -432,15 +438,15 @@ def qkv_norm_rope(x: DeviceTensor, heads: int, kv_heads: int, dim: int, position
                x.ctx.empty((n, tokens, kv_heads, dim), dtype))
     q, k, v = out
     kind = (q or k or v).dtype
-    q_at, k_at, v_at = (_at(t, (n, tokens, h, dim), kind, what)
+    q_at, k_at, v_at = (_at(t, (n, tokens, h, dim), kind, what, x.ctx)
                         for t, h, what in ((q, heads, "q"), (k, kv_heads, "k"), (v, kv_heads, "v")))
     items, positions_at = 1, None
     if positions is not None:
         items = positions.shape[0] if len(positions.shape) == 3 else 1
-        positions_at = _at(positions, (items,) * (len(positions.shape) - 2) + (tokens, 3), _F32, "positions")
+        positions_at = _at(positions, (items,) * (len(positions.shape) - 2) + (tokens, 3), _F32, "positions", x.ctx)
     check(lib().mbx_qkv_norm_rope(x.ctx.handle, x.ptr, _storage(x), n, tokens, stride, heads, kv_heads, dim, norm,
-                                  _at(q_gamma, (dim,), _F32, "q_gamma"), _at(k_gamma, (dim,), _F32, "k_gamma"), eps,
-                                  positions_at, items, _Int64x3(*axis_dims), theta, PAIRINGS[pairing], q_at, k_at,
+                                  _at(q_gamma, (dim,), _F32, "q_gamma", x.ctx),
+                                  _at(k_gamma, (dim,), _F32, "k_gamma", x.ctx), eps, positions_at, items, _Int64x3(*axis_dims), theta, PAIRINGS[pairing], q_at, k_at,
                                   v_at, _STORAGE.get(kind, -1)))
     return out
 
@@ -456,6 +462,7 @@ def _heads(q: DeviceTensor, k: DeviceTensor):
         raise ValueError("expected q [n, nq, heads, dim] and k [n, nk, kv_heads, dim]")
     if q.dtype is not k.dtype and q.dtype != k.dtype:
         raise ValueError("q and k differ in type")
+    _near(k, q.ctx, "k")
     return n, nq, nk, heads, kv_heads, dim
 
 
@@ -487,9 +494,10 @@ def block_select(q: DeviceTensor, k: DeviceTensor, topk: int, block_k: int = 64,
     n, nq, nk, heads, kv_heads, dim = _heads(q, k)
     shape = (n, heads, -(-nq // abi.ATTENTION_BLOCK_Q), topk)
     out = out or q.ctx.empty(shape, np.int32)
-    _fits(out, shape, _I32, "out")
-    mask_at = _at(key_mask, (n, nk), _U8, "key_mask")
+    _fits(out, shape, _I32, "out", q.ctx)
+    mask_at = _at(key_mask, (n, nk), _U8, "key_mask", q.ctx)
     workspace = workspace or _own_scratch(q.ctx, block_select_workspace, q, k, block_k)
+    _near(workspace, q.ctx, "workspace")
     check(lib().mbx_block_select(q.ctx.handle, q.ptr, heads * dim if q_stride is None else q_stride, k.ptr,
                                  kv_heads * dim if k_stride is None else k_stride, _storage(q), n, nq, nk, heads,
                                  kv_heads, dim, block_k, mask_at, topk, out.ptr, workspace.ptr, workspace.nbytes))
@@ -515,12 +523,13 @@ def block_attention(q: DeviceTensor, k: DeviceTensor, v: DeviceTensor, index: De
     among the same 16 keys."""
     n, nq, nk, heads, kv_heads, dim = _heads(q, k)
     topk = index.shape[-1]
-    _fits(v, k.shape, k.dtype, "v")
-    _fits(index, (n, heads, -(-nq // abi.ATTENTION_BLOCK_Q), topk), _I32, "index")
-    mask_at = _at(key_mask, (n, nk), _U8, "key_mask")
+    _fits(v, k.shape, k.dtype, "v", q.ctx)
+    _fits(index, (n, heads, -(-nq // abi.ATTENTION_BLOCK_Q), topk), _I32, "index", q.ctx)
+    mask_at = _at(key_mask, (n, nk), _U8, "key_mask", q.ctx)
     out = out or q.ctx.empty(q.shape, q.dtype)
-    _fits(out, q.shape, q.dtype, "out")
+    _fits(out, q.shape, q.dtype, "out", q.ctx)
     workspace = workspace or _own_scratch(q.ctx, block_attention_workspace, q, k, index, block_k)
+    _near(workspace, q.ctx, "workspace")
     kv_row = kv_heads * dim
     check(lib().mbx_block_attention(q.ctx.handle, q.ptr, heads * dim if q_stride is None else q_stride, k.ptr,
                                     kv_row if k_stride is None else k_stride, v.ptr,

@@ -162,6 +162,39 @@ def test_python_front_end_refuses_mismatched_tensors(mbx):
                           out=(t((1, 4, 2, 16)), t((1, 4, 1, 16)), t((1, 4, 1, 16))))
 
 
+def test_python_front_end_refuses_tensors_of_another_device(mbx):
+    class Device:  # a context, as far as the checks look into it
+        def __init__(self, device):
+            self.device, self.handle = device, None
+    here, same, other = Device(0), Device(0), Device(1)
+
+    def t(ctx, shape, dtype=np.float16):
+        return mbx.DeviceTensor.wrap(ctx, A, shape, dtype=dtype)
+    shapes = dict(q=(1, 4, 2, 16), k=(1, 5, 1, 16), v=(1, 5, 1, 16), index=(1, 2, 1, 3), key_mask=(1, 5),
+                  workspace=(8,), out=(1, 4, 2, 16))
+    kinds = dict(index=np.int32, key_mask=np.uint8, workspace=np.uint8)
+
+    def attend(**at):
+        a = {s: t(at.get(s, here), shape, kinds.get(s, np.float16)) for s, shape in shapes.items()}
+        return mbx.block_attention(a.pop("q"), a.pop("k"), a.pop("v"), a.pop("index"), **a)
+
+    def select(**at):
+        a = {s: t(at.get(s, here), shapes[s], kinds.get(s, np.float16)) for s in ("q", "k", "key_mask", "workspace")}
+        return mbx.block_select(a.pop("q"), a.pop("k"), 3, out=t(at.get("out", here), shapes["index"], np.int32), **a)
+
+    def rope(**at):
+        parts = tuple(t(at.get(s, here), (1, 4, h, 16)) for s, h in (("q", 2), ("k", 1), ("v", 1)))
+        return mbx.qkv_norm_rope(t(here, (1, 4, 64)), 2, 1, 16, positions=t(at.get("positions", here), (4, 3), np.float32),
+                                 q_gamma=t(at.get("q_gamma", here), (16,), np.float32), out=parts)
+    for call, names in ((attend, shapes), (select, ("q", "k", "key_mask", "workspace", "out")),
+                        (rope, ("q", "k", "v", "positions", "q_gamma"))):
+        for name in names:
+            with pytest.raises(ValueError, match="device"):
+                call(**{name: other})
+            with pytest.raises(mbx.MbxError, match="context"):  # past the front end: there is no handle
+                call(**{name: same})
+
+
 def test_tensor_size_is_a_plain_integer(mbx):
     """A shape of NumPy's narrow integers must not wrap around (or warn) on its way to a size in bytes."""
     t = mbx.DeviceTensor(None, (np.int32(1 << 16), np.int32(1 << 16), np.uint8(3)), ptr=A)
