@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a) {
     }
 }
 
-constexpr int64_t kSms = 148;
+constexpr int64_t kSms = 148;  // of a B200: the workspace functions have no context to ask
 
 // Which kernel takes a problem, and over how many CTAs a list is split.
 struct Plan {

@@ -341,13 +341,13 @@ void launch_means(mbx_ctx* ctx, const MeanArgs& a, int64_t n) {
 }
 
 MeanSide mean_side(const void* x, int dtype, int64_t stride, int64_t rows, int block, int blocks, int64_t width,
-                   const uint8_t* mask, double* mean, uint8_t* live, int64_t n) {
+                   const uint8_t* mask, double* mean, uint8_t* live, int64_t n, int sms) {
     MeanSide m{x, stride, rows, block, blocks, (int)width, 0, 0, mask, mean, live};
     // 64 pieces (a KB) of a row for a CTA, evenly; 32 where that leaves fewer than four CTAs an SM. A CTA's fixed
     // costs want long columns (65536 x 16 x 128 bf16: 217 us in all with 32, 202 with 64, 200 with 128), a small
     // problem many CTAs (2 x 1961 and 4133 x 80 f32: 25 us with 32, 27 with 64, 34 with 128).
     const int pieces = (int)width / (dtype == MBX_DTYPE_F32 ? 4 : 8);
-    const int most = n * blocks * ((pieces + 63) / 64) < 4 * 148 ? 32 : 64;
+    const int most = n * blocks * ((pieces + 63) / 64) < 4 * sms ? 32 : 64;
     m.groups = (pieces + most - 1) / most;
     m.cols = (pieces + m.groups - 1) / m.groups;
     return m;
@@ -389,9 +389,9 @@ void launch_block_select(mbx_ctx* ctx, const BlockShape& s, const void* q, int64
     if (kb > 0) {
         MeanArgs m{};
         m.side[0] = mean_side(q, s.dtype, q_stride, s.nq, MBX_ATTENTION_BLOCK_Q, qb, s.heads * s.dim, nullptr,
-                              reinterpret_cast<double*>(ws + l.qm), nullptr, s.n);
+                              reinterpret_cast<double*>(ws + l.qm), nullptr, s.n, ctx->sm_count);
         m.side[1] = mean_side(k, s.dtype, k_stride, s.nk, (int)s.block_k, kb, s.kv_heads * s.dim, key_mask,
-                              reinterpret_cast<double*>(ws + l.km), ws + l.live, s.n);
+                              reinterpret_cast<double*>(ws + l.km), ws + l.live, s.n, ctx->sm_count);
         if (s.dtype == MBX_DTYPE_F32)
             launch_means<float>(ctx, m, s.n);
         else if (s.dtype == MBX_DTYPE_F16)

@@ -55,7 +55,7 @@ __device__ __forceinline__ float4 f4_fma(float4 a, float4 b, float4 c) {
     return make_float4(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y), fmaf(a.z, b.z, c.z), fmaf(a.w, b.w, c.w));
 }
 
-// Two f32 in one register pair: sm_100 adds and multiplies both in one instruction, each as if alone.
+// Two f32 in one register pair: sm_100 adds both, or multiplies and adds both, in one instruction, each as if alone.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t v;
     asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
@@ -72,11 +72,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 
