@@ -50,6 +50,8 @@ extern "C" {
 #define MBX_DTYPE_F16 1
 /* Storage of the image-token attention operators only (no weights). */
 #define MBX_DTYPE_BF16 2
+/* mbx_block_attention: added to the dtype of 16-bit operands, out is float32 (what mbx_conv1x1 reads). */
+#define MBX_OUT_F32 16
 
 /* Channels that a rotation turns together: (2i, 2i + 1), or (i, i + D/2) of a section of D channels. */
 #define MBX_ROPE_ADJACENT 0
@@ -344,8 +346,8 @@ int32_t mbx_block_select(mbx_ctx *ctx, const void *q, int64_t q_stride, const vo
  * layout, from there or from the caller) and that key_mask keeps. Entries outside
  * [0, ceil(nk / block_k)) are skipped; a block listed twice counts twice. A row with no key left
  * is zero. Masked keys and values may hold anything, and so may those of blocks that no list names; the
- * others are finite. dim <= 128; q, k, v and out have the same dtype. 16-bit weights are rounded to that type
- * before the product with v. Many query rows of float32 are carried as two float16 parts of every value, at one
+ * others are finite. dim <= 128; q, k and v have the same dtype, and so has out, or float32 with
+ * dtype | MBX_OUT_F32. 16-bit weights are rounded to the operands' type before the product with v. Many query rows of float32 are carried as two float16 parts of every value, at one
  * power of two for each query row's head and for each 16 keys of a head of k and of v: a value is held to 2^-22
  * of itself or 2^-39 of the largest of those, whichever is more.
  * out must not overlap an input. workspace as for mbx_block_select (the size may be 0, and

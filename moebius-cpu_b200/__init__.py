@@ -516,24 +516,29 @@ def block_attention_workspace(q: DeviceTensor, k: DeviceTensor, index: DeviceTen
 def block_attention(q: DeviceTensor, k: DeviceTensor, v: DeviceTensor, index: DeviceTensor, block_k: int = 64,
                     key_mask: Optional[DeviceTensor] = None, scale: Optional[float] = None,
                     q_stride: Optional[int] = None, k_stride: Optional[int] = None, v_stride: Optional[int] = None,
-                    workspace: Optional[DeviceTensor] = None, out: Optional[DeviceTensor] = None) -> DeviceTensor:
+                    workspace: Optional[DeviceTensor] = None, out: Optional[DeviceTensor] = None,
+                    out_dtype=None) -> DeviceTensor:
     """softmax(scale q k^T) v over the key blocks that index lists for each 128 query rows (mbx_block_attention);
     scale is 1 / sqrt(dim) by default. Masked keys, and blocks that no list names, may hold anything. 16-bit weights are
     rounded to the type before the product with v; float32 is held to 2^-22 of a value, or 2^-39 of the largest of its head
-    among the same 16 keys."""
+    among the same 16 keys. The result has q's type, or is float32 (out_dtype, or out's own type) for the projection
+    behind."""
     n, nq, nk, heads, kv_heads, dim = _heads(q, k)
     topk = index.shape[-1]
     _fits(v, k.shape, k.dtype, "v", q.ctx)
     _fits(index, (n, heads, -(-nq // abi.ATTENTION_BLOCK_Q), topk), _I32, "index", q.ctx)
     mask_at = _at(key_mask, (n, nk), _U8, "key_mask", q.ctx)
-    out = out or q.ctx.empty(q.shape, q.dtype)
-    _fits(out, q.shape, q.dtype, "out", q.ctx)
+    out = out or q.ctx.empty(q.shape, q.dtype if out_dtype is None else out_dtype)
+    dtype = _storage(q)
+    if out.dtype is _F32 or out.dtype == _F32:
+        dtype |= abi.OUT_F32
+    _fits(out, q.shape, _F32 if dtype & abi.OUT_F32 else q.dtype, "out", q.ctx)
     workspace = workspace or _own_scratch(q.ctx, block_attention_workspace, q, k, index, block_k)
     _near(workspace, q.ctx, "workspace")
     kv_row = kv_heads * dim
     check(lib().mbx_block_attention(q.ctx.handle, q.ptr, heads * dim if q_stride is None else q_stride, k.ptr,
                                     kv_row if k_stride is None else k_stride, v.ptr,
-                                    kv_row if v_stride is None else v_stride, _storage(q), n, nq, nk, heads, kv_heads,
+                                    kv_row if v_stride is None else v_stride, dtype, n, nq, nk, heads, kv_heads,
                                     dim, block_k, mask_at, index.ptr, topk,
                                     1.0 / math.sqrt(dim) if scale is None else scale, out.ptr, workspace.ptr,
                                     workspace.nbytes))

@@ -30,6 +30,7 @@ ERR_TIMEOUT = 9
 DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
+OUT_F32 = 16
 
 ROPE_ADJACENT = 0
 ROPE_HALVES = 1

@@ -13,6 +13,7 @@ struct AttnArgs {
     const int32_t* index;  // [n][heads][q_blocks][topk]
     float scale;           // scale · log2(e): exponentials are 2^x
     void* out;             // [n][nq][heads][dim]
+    bool out_f32;          // float32, whatever the operands' type
     float* part;           // splits > 1: [n][nq][heads][splits][dim + 4]: Σ p v, log2 of what p is relative to, Σ p, 2 unused
     int splits;            // CTAs that share a list
 };

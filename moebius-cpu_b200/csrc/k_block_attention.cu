@@ -22,6 +22,14 @@
 namespace mbx {
 namespace {
 
+template <class T>
+__device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, float v) {
+    if (a.out_f32)
+        static_cast<float*>(a.out)[at] = v;
+    else
+        static_cast<T*>(a.out)[at] = (T)v;
+}
+
 constexpr int kRowWarps = 4;
 constexpr int kListPart = 1024;  // list entries in shared memory at a time
 
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const At
         }
         const int64_t row = (item * a.nq + r0 + r) * a.heads + h;
         if (a.splits == 1) {
-            static_cast<T*>(a.out)[row * a.dim + ch] = (T)(sum == 0.0f ? 0.0f : o / sum);
+            store_out<T>(a, row * a.dim + ch, sum == 0.0f ? 0.0f : o / sum);
         } else {
             float* p = a.part + (row * a.splits + split) * (a.dim + 4);
             p[ch] = o;
@@ -232,7 +240,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttnArgs a) {
     if ((int)threadIdx.x < a.dim) {
         const float* x = reinterpret_cast<const float*>(acc);
         const float y = (x[threadIdx.x] + x[128 + threadIdx.x]) + (x[256 + threadIdx.x] + x[384 + threadIdx.x]);
-        static_cast<T*>(a.out)[(int64_t)blockIdx.x * a.dim + threadIdx.x] = (T)(total == 0.0f ? 0.0f : y / total);
+        store_out<T>(a, (int64_t)blockIdx.x * a.dim + threadIdx.x, total == 0.0f ? 0.0f : y / total);
     }
 }
 
@@ -311,7 +319,8 @@ size_t block_attention_bytes(const BlockShape& s, int64_t topk) {
 
 void launch_block_attention(mbx_ctx* ctx, const BlockShape& s, const void* q, int64_t q_stride, const void* k,
                             int64_t k_stride, const void* v, int64_t v_stride, const uint8_t* key_mask,
-                            const int32_t* index, int64_t topk, float scale, void* out, void* workspace) {
+                            const int32_t* index, int64_t topk, float scale, void* out, bool out_f32,
+                            void* workspace) {
     const Plan p = plan_of(s, topk);
     AttnArgs a{};
     a.q = q, a.k = k, a.v = v;
@@ -322,7 +331,7 @@ void launch_block_attention(mbx_ctx* ctx, const BlockShape& s, const void* q, in
     a.q_blocks = (int)((s.nq + MBX_ATTENTION_BLOCK_Q - 1) / MBX_ATTENTION_BLOCK_Q);
     a.mask = key_mask, a.index = index;
     a.scale = scale * 1.4426950408889634f;  // log2(e)
-    a.out = out;
+    a.out = out, a.out_f32 = out_f32;
     a.part = static_cast<float*>(workspace);
     a.splits = p.splits;
     if (p.rows) {

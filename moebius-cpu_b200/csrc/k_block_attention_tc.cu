@@ -629,6 +629,8 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                     if (!store || i + g >= a.dim) continue;
                     if (a.splits > 1)
                         store8(part + i + g, y);
+                    else if (!SPLIT && a.out_f32)
+                        store8(static_cast<float*>(a.out) + at * a.dim + i + g, y);
                     else
                         store8(static_cast<OUT*>(a.out) + at * a.dim + i + g, y);
                 }

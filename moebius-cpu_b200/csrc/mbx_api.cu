@@ -873,7 +873,7 @@ int32_t mbx_block_attention_workspace(int32_t dtype, int64_t n, int64_t nq, int6
                                       int64_t kv_heads, int64_t dim, int64_t block_k, int64_t topk, size_t* bytes) {
     return guard([&] {
         require_ptr(bytes, "bytes");
-        const mbx::BlockShape s = block_shape(dtype, n, nq, nk, heads, kv_heads, dim, block_k, 128);
+        const mbx::BlockShape s = block_shape(dtype & ~MBX_OUT_F32, n, nq, nk, heads, kv_heads, dim, block_k, 128);
         require_topk(s, topk);
         *bytes = mbx::block_attention_bytes(s, topk);
     });
@@ -886,6 +886,8 @@ int32_t mbx_block_attention(mbx_ctx* ctx, const void* q, int64_t q_stride, const
                             size_t workspace_bytes) {
     return guard([&] {
         require_ctx(ctx);
+        const int32_t out_dtype = dtype & MBX_OUT_F32 ? MBX_DTYPE_F32 : dtype;
+        dtype &= ~MBX_OUT_F32;
         const mbx::BlockShape s = block_shape(dtype, n, nq, nk, heads, kv_heads, dim, block_k, 128);
         require_topk(s, topk);
         require_rows(q, q_stride, heads * dim, dtype, "q");
@@ -897,7 +899,7 @@ int32_t mbx_block_attention(mbx_ctx* ctx, const void* q, int64_t q_stride, const
         require_aligned(out, 16, "out");
         if (nk == 0 || topk == 0) {  // no key for any row
             use_device(ctx);
-            check_cuda(cudaMemsetAsync(out, 0, (size_t)(n * nq * heads * dim) * storage_size(dtype), ctx->stream),
+            check_cuda(cudaMemsetAsync(out, 0, (size_t)(n * nq * heads * dim) * storage_size(out_dtype), ctx->stream),
                        "cudaMemsetAsync");
             return;
         }
@@ -907,7 +909,7 @@ int32_t mbx_block_attention(mbx_ctx* ctx, const void* q, int64_t q_stride, const
         require_workspace(workspace, workspace_bytes, mbx::block_attention_bytes(s, topk));
         use_device(ctx);
         mbx::launch_block_attention(ctx, s, q, q_stride, k, k_stride, v, v_stride, key_mask, index, topk, scale, out,
-                                    workspace);
+                                    out_dtype == MBX_DTYPE_F32, workspace);
     });
 }
 

@@ -199,7 +199,7 @@ void launch_block_select(mbx_ctx* ctx, const BlockShape& s, const void* q, int64
                          int64_t k_stride, const uint8_t* key_mask, int64_t topk, int32_t* index, void* workspace);
 void launch_block_attention(mbx_ctx* ctx, const BlockShape& s, const void* q, int64_t q_stride, const void* k,
                             int64_t k_stride, const void* v, int64_t v_stride, const uint8_t* key_mask,
-                            const int32_t* index, int64_t topk, float scale, void* out, void* workspace);
+                            const int32_t* index, int64_t topk, float scale, void* out, bool out_f32, void* workspace);
 
 // λ layers (k_lambda.cu). lambda_content needs scratch: pmax and psum
 // [items][chunks][k], plam [items][chunks][k][vd] with chunks = lambda_chunks(rows).

@@ -598,3 +598,46 @@ def test_a_captured_call_needs_its_own_workspace(mbx):
         ctx.set_stream(None)
         assert not ctx.capturing
         del graph
+
+
+@pytest.mark.parametrize("kind", DTYPES)
+@pytest.mark.parametrize("nq,heads", [(1, 1), (1, 70), (140, 2), (140, 148)])  # rows, split rows, split and whole lists
+def test_block_attention_to_float32(mbx, ctx, kind, nq, heads):
+    """The result of any operands before it is rounded to their type, and zeros where no key is."""
+    rng = np.random.default_rng(53)
+    q, k, v, mask, index = attend_inputs(rng, 2, nq, 500, heads, 1, 40, 32, 9, "empty", kind)
+    out = mbx.block_attention(*(up(ctx, t) for t in (q, k, v, index)), block_k=32, key_mask=up(ctx, mask),
+                              out_dtype=np.float32)
+    assert out.dtype == np.float32
+    want, tol = ref.attention(*(ref.wide(t) for t in (q, k, v)), index, 32, mask, 40 ** -0.5, kind)
+    # Less the rounding that ref.attention counts for the operands' type, (|o| + t) of HALF_STEP, and with f32's.
+    half = ref.HALF_STEP[kind]
+    tol = (tol - ref.TINY[kind] - half * np.abs(want)) / (1 + half)
+    close(out.numpy(), want, np.maximum(tol, 0) + 2.0 ** -24 * np.abs(want) + ref.TINY["f32"])
+    none = ctx.empty((2, 0, 1, 40), q.dtype)
+    index = up(ctx, np.zeros((2, heads, -(-nq // 128), 1), np.int32))
+    given = up(ctx, np.full(q.shape, 7.0, np.float32))
+    assert not mbx.block_attention(up(ctx, q), none, none, index, out=given).numpy().any()
+
+
+@pytest.mark.parametrize("kind", DTYPES)
+def test_the_operators_between_two_projections(mbx, ctx, oracle, kind):
+    """From one 1x1 convolution to the next in every type: the attention hands float32 on."""
+    rng = np.random.default_rng(59)
+    n, h, w, c, heads, dim = 1, 12, 20, 64, 4, 32
+    x = rng.standard_normal((n, h, w, c)).astype(np.float32)
+    weights = [(rng.standard_normal(s) / 9).astype(np.float32) for s in ((3 * heads * dim, c), (c, heads * dim))]
+    p_in, p_out = (mbx.Param(ctx, t) for t in weights)
+    d = up(ctx, x)
+    qkv = mbx.conv1x1(d, p_in)
+    rows = mbx.DeviceTensor.wrap(ctx, qkv.ptr, (n, h * w, p_in.c_out))
+    q, k, v = mbx.qkv_norm_rope(rows, heads, heads, dim, dtype=ref.KINDS[kind])
+    index = mbx.block_select(q, k, 5, block_k=32)
+    o = mbx.block_attention(q, k, v, index, block_k=32, out_dtype=np.float32)
+    y = mbx.conv1x1(mbx.DeviceTensor.wrap(ctx, o.ptr, (n, h, w, heads * dim)), p_out, residual=d)
+    want = oracle.conv1x1(o.numpy().reshape(n, h, w, -1), weights[1], None, x)
+    assert max_rel_err(y.numpy(), want) <= 1e-5
+    attended, tol = ref.attention(*(ref.wide(t.numpy()) for t in (q, k, v)), index.numpy(), 32, None, dim ** -0.5, kind)
+    close(o.numpy(), attended, tol)
+    p_in.close()
+    p_out.close()
