@@ -641,3 +641,71 @@ def test_the_operators_between_two_projections(mbx, ctx, oracle, kind):
     close(o.numpy(), attended, tol)
     p_in.close()
     p_out.close()
+
+
+@pytest.mark.parametrize("kind", DTYPES)
+@pytest.mark.parametrize("nk", [1, 2, 15, 17])
+def test_block_attention_of_few_keys_for_many_rows(mbx, ctx, kind, nk):
+    rng = np.random.default_rng(61)
+    for dim in (40, 96):
+        q, k, v, _, index = attend_inputs(rng, 2, 200, nk, 2, 1, dim, 16, 3, "none", kind)
+        out = mbx.block_attention(*(up(ctx, t) for t in (q, k, v, index)), block_k=16)
+        want, tol = ref.attention(*(ref.wide(t) for t in (q, k, v)), index, 16, None, dim ** -0.5, kind)
+        close(out.numpy(), want, tol)
+
+
+@pytest.mark.parametrize("kind", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_full_card_repeats_itself(mbx, ctx, kind, dim):
+    """Several waves of CTAs, two an SM, give the same bits every time."""
+    rng = np.random.default_rng(67)
+    q, k, v = (up(ctx, ref.narrow(rng.standard_normal((2, 4096, h, dim)), kind)) for h in (16, 8, 8))
+    index = mbx.block_select(q, k, 16, block_k=32)
+    first = mbx.block_attention(q, k, v, index, block_k=32).numpy().tobytes()
+    for _ in range(5):
+        assert mbx.block_select(q, k, 16, block_k=32).numpy().tobytes() == index.numpy().tobytes()
+        assert mbx.block_attention(q, k, v, index, block_k=32).numpy().tobytes() == first
+
+
+@pytest.mark.skipif(importlib.util.find_spec("torch") is None, reason="captures with torch")
+def test_a_captured_layer(mbx):
+    """Heads, choice and attention in one graph, replayed on new inputs."""
+    import torch
+    rng = np.random.default_rng(71)
+    n, tokens, heads, kv, dim = 2, 300, 4, 2, 40
+    with mbx.Context(0) as ctx:
+        x = ctx.empty((n, tokens, (heads + 2 * kv) * dim))
+        pos = rng.integers(0, 30, (tokens, 3)).astype(np.float32)
+        at = up(ctx, pos)
+        parts = tuple(ctx.empty((n, tokens, h, dim), np.float16) for h in (heads, kv, kv))
+        index, out = ctx.empty((n, heads, 3, 5), np.int32), ctx.empty(parts[0].shape)
+        ws = mbx.block_select_workspace(parts[0], parts[1], 32), mbx.block_attention_workspace(parts[0], parts[1], index, 32)
+
+        def call():
+            mbx.qkv_norm_rope(x, heads, kv, dim, positions=at, axis_dims=(0, 20, 20), pairing="halves", out=parts)
+            mbx.block_select(parts[0], parts[1], 5, block_k=32, workspace=ws[0], out=index)
+            mbx.block_attention(*parts, index, block_k=32, workspace=ws[1], out=out)
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        ctx.synchronize()
+        ctx.set_stream(stream.cuda_stream)
+        call()
+        ctx.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            call()
+        for _ in range(2):
+            host = rng.standard_normal(x.shape).astype(np.float32)
+            mbx.check(mbx.abi.lib().mbx_memcpy_h2d(ctx.handle, x.vp, host.ctypes.data_as(ctypes.c_void_p), host.nbytes))
+            ctx.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            torch.cuda.synchronize()
+            wide = host.astype(np.float64).reshape(n, tokens, -1, dim)
+            for got, part in zip(parts, (wide[:, :, :heads], wide[:, :, heads:heads + kv])):
+                y, size = ref.norm_rope(part, None, 1e-6, True, pos[None], (0, 20, 20), 10000.0, True)
+                close(got.numpy(), y, rope_tolerance(y, size, "f16"))
+            q, k, v = (ref.wide(t.numpy()) for t in parts)
+            assert np.array_equal(index.numpy(), ref.select(q, k, 5, 32))
+            want, tol = ref.attention(q, k, v, index.numpy(), 32, None, dim ** -0.5, "f16")
+            close(out.numpy(), want, tol)
+        ctx.set_stream(None)
+        del graph
