@@ -255,10 +255,10 @@ struct Plan {
 
 Plan plan_of(const BlockShape& s, int64_t topk) {
     Plan p{};
-    // 16 bits: the rows kernel for one or two rows of few heads (16 heads x 128 over 4096 of 65536 keys bf16: 14 us against
-    // 21, four rows 29 against 21; 128 heads: 72 us against 63). f32: while it reads no more than twice the keys that the tensor cores' operands would have to
-    // be split for (the same shape, 32 rows: 141 us against 238, 64: 240 against 240; 16 x 1024 of 4096 keys x 8 x 40, 32
-    // rows: 100 against 108, 64: 190 against 112).
+    // 16 bits: the rows kernel for one or two rows of few heads (16 heads x 128 over 4096 of 65536 keys bf16: 14.5 us
+    // against 16.5, four rows 26 against 16; 128 heads: 72 us against 61). f32: while it reads no more than twice the keys
+    // that the tensor cores' operands would have to be split for (the same shape, 32 rows: 127 us against 221, 64: 207
+    // against 222; 16 x 1024 of 4096 keys x 8 x 40, 16 rows: 70 against 103, 32: 117 against 105, 64: 199 against 110).
     const bool few = s.dtype == MBX_DTYPE_F32
                          ? (s.nq + 3) / 4 * s.heads * std::min(topk * s.block_k, s.nk) <= 2 * s.nk * s.kv_heads
                          : s.nq <= 2 && s.n * s.heads < 64;

@@ -23,8 +23,10 @@
 // Shared memory: Q, K and V in 128-byte-swizzled panels of 64 channels; V serves as the N-major
 // operand as it lies, so nothing is transposed.
 //
-// 16-bit operands: P is rounded to their type (half a step of a weight, beside half a step of the
-// result at the end). The weights are relative to a reference that is raised only when a row's
+// 16-bit operands: P is rounded to their type: half a step of a weight, beside half a step of the
+// result at the end (2.16e-4 of the exact result at 1024 px and 1.73e-3 for video, where the result's rounding
+// alone is 2.07e-4 and 1.66e-3). Exact weights would be two parts of each, half as many tensor products again in a
+// kernel that is bound by them and by the instructions that make the weights. The weights are relative to a reference that is raised only when a row's
 // maximum outgrows it by 2^8, so O, which accumulates in TMEM over the whole list, is rarely
 // rescaled.
 //
@@ -44,9 +46,11 @@
 //
 // Masked keys: S becomes −inf; their V rows become zero in shared memory (16-bit) or while
 // splitting (f32), since zero times what a mask hides may be NaN.
-// Measured on a B200: 32768 queries x 16 heads x 128 bf16 over 2048 keys each in 522 us (1050 TFLOP/s; tensor cores
-// 53 % busy, exponentials 54 %), 2 x 16384 x 16 x 64 f16 over 2048 keys in 414 us (664 TFLOP/s; exponentials 63 %),
-// 16 x 4096 x 8 x 40 f32 over 1024 keys in 477 us with the split (180 TFLOP/s, 540 in products).
+// Measured on a B200, in a burst of ten calls and in a run of two seconds, in which the card clocks down:
+// 32768 queries x 16 heads x 128 bf16 over 2048 keys each in 527 and 612 us (1043 and 898 TFLOP/s; tensor cores
+// 50 % busy, exponentials 51 %), 2 x 16384 x 16 x 64 f16 over 2048 keys in 421 and 441 us (653 and 624 TFLOP/s;
+// exponentials 61 %), 16 x 4096 x 8 x 40 f32 over 1024 keys in 494 and 548 us with the split (174 and 157 TFLOP/s,
+// three times that in products).
 // Every wait is bounded; on timeout the CTA records the error, waits (bounded) for its copies and
 // MMAs in flight, frees TMEM and returns. It looks for them when every warp has stopped: a producer may be through
 // with its part before another warp gives up.

@@ -17,7 +17,8 @@
 // block computes each once into shared memory and a lane keeps its channels' in registers while it walks the
 // token's heads. Pairs of halves meet through shared memory, nine floats a lane against bank conflicts.
 // Measured on a B200: 65536 tokens x 32 heads x 128 bf16 in 213 us (5.0 TB/s read and written, instructions
-// issued in 63 % of the cycles), 65536 x 24 x 40 f32 -> f16 in 100 us (3.8 TB/s, 62 %).
+// issued in 60 % of the cycles), 65536 x 24 x 40 f32 -> f16 in halves in 100 us (3.8 TB/s, 62 %). Four blocks an SM
+// leave 64 registers a thread, of which halves spill 2 to 6.
 // Angles: theta^(−2i / D_a) / 2π and its product with the position are f64, as
 // an f32 product is off by 6e-8 of the angle, 0.06 rad at a position of 1e6;
 // the part behind the whole turns then fits f32, and sincospif takes it.
