@@ -28,7 +28,9 @@
 // alone is 2.07e-4 and 1.66e-3). Exact weights would be two parts of each, half as many tensor products again in a
 // kernel that is bound by them and by the instructions that make the weights. The weights are relative to a reference that is raised only when a row's
 // maximum outgrows it by 2^8, so O, which accumulates in TMEM over the whole list, is rarely
-// rescaled.
+// rescaled. The reference comes off S before the factor: as one fused step, its own product is rounded to a
+// step of f32, which past logits of 2^24 is more than one and past 2^27 more than f16's weights can hold
+// (0.7 to 3.5 % of the time; a branch for large references cost as much).
 //
 // f32 operands: two f16 parts of every value after a power-of-two scale, each 16 keys of a head of k and
 // of v with one of their own (beforehand, attention_split_kernel), each query row with its own (as its CTA
@@ -37,7 +39,7 @@
 // whole), and the weights in two parts after a scale of 2^7. The scales of k go into the factor of the
 // exponents, those of v into what the weights are relative to: with x = log2 of a weight and 2^e the scale of
 // its v, O gathers 2^(x − e − m) times the scaled v, m being the running maximum of x − e, while the sum of
-// weights has a maximum of its own. Both are whole numbers, so every rescaling is exact.
+// weights is relative to that of x. Both are whole numbers, so every rescaling is exact.
 // The tensor core truncates as it adds into its f32 accumulator, so a long sum there drifts by about 2^-25 a
 // step: the softmax threads add each tile's P·V to a second set of TMEM columns, rounding to nearest, and the
 // next tile begins a fresh sum. (16 x 4096 x 8 x 40 over 1024 keys, relative to the exact result: 3.0e-7 in
@@ -74,7 +76,7 @@ constexpr float kLazy = 8.0f;   // log2 of the largest weight
 constexpr int kWeightExp = 7;   // f32 operands: weights are scaled by 2^7 before their split, up to 2^15
 constexpr int kScaleExp = 14;   // f32 operands: the largest magnitude is scaled to [2^14, 2^15)
 constexpr int kChunk = 16;      // f32 operands: keys that share a scale; every block is a multiple
-constexpr float kNone = -1e30f;  // f32 operands: the running maxima before the first key
+constexpr float kNone = -1e30f;  // f32 operands: the running maximum before the first key
 
 struct TcArgs {
     AttnArgs a;
@@ -427,9 +429,9 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             c = ldexpf(c, -scale_exponent(q_top[threadIdx.x]));
         }
         if (!SPLIT) c = fmaxf(c, 1.17549435e-38f);  // f32: with the scale of k in it
-        // What the weights are relative to, in units of S, and their sum. f32: log2 of what O is relative to, and of what
-        // the sum is.
-        float ref = SPLIT ? kNone : -INFINITY, l = 0.0f, ref_l = kNone;
+        // What the weights are relative to, in units of S, and their sum. f32: log2 of what the sum is relative to, and of
+        // what O is, relative to that.
+        float ref = SPLIT ? kNone : -INFINITY, l = 0.0f, off_o = 0.0f;
         // O's columns, 16 at a time, as far as there are channels.
         auto columns = [&](auto&& f) {
 #pragma unroll
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                 }
             }
             constexpr int CHUNKS = SPLIT ? 4 : 1;
-            float cs[CHUNKS];  // factor of S in the exponent
+            float cs[CHUNKS], raw[CHUNKS];  // factor of S in the exponent; f32: the largest S, and in t times the factor
             float top, top_o = 0.0f;
             bool raise;
             if constexpr (SPLIT) {
@@ -478,10 +480,11 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     cs[u] = fmaxf(c * fks[u], 1.17549435e-38f);
+                    raw[u] = t[u];
                     t[u] *= cs[u];
-                    top = fmaxf(top, t[u]), top_o = fmaxf(top_o, t[u] - es[u]);
+                    top = fmaxf(top, t[u]), top_o = fmaxf(top_o, t[u] - ref - es[u]);
                 }
-                raise = top_o - ref > kLazy || top - ref_l > kLazy;
+                raise = top - ref > kLazy || top_o - off_o > kLazy;
             } else {
                 cs[0] = c;
                 top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
@@ -491,15 +494,16 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             if (__any_sync(0xffffffffu, raise)) {
                 float f = 1.0f;
                 if constexpr (SPLIT) {
-                    if (top_o - ref > kLazy) {
-                        const float up = ceilf(top_o);
-                        f = pow2(ref - up);
-                        ref = up;
-                    }
-                    if (top - ref_l > kLazy) {
-                        const float up = ceilf(top);
-                        l *= pow2(ref_l - up);
-                        ref_l = up;
+                    if (raise) {
+                        const float4 e = *reinterpret_cast<const float4*>(v_exp[slot]);
+                        const float es[4] = {e.x, e.y, e.z, e.w};
+                        const float up = top - ref > kLazy ? ceilf(top) : ref, was = fmaxf(off_o - (up - ref), -1000.0f);
+                        l *= pow2(ref - up);
+                        ref = up, off_o = was;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            if (t[u] - ref - es[u] - was > kLazy) off_o = fmaxf(off_o, ceilf(t[u] - ref - es[u]));
+                        f = pow2(was - off_o);
                     }
                 } else {
                     if (raise) {
@@ -530,16 +534,21 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
                 if (!ok) break;
                 tc_fence_after();
             }
-            float mc[CHUNKS];  // log2 of what a chunk's weights are relative to
+            // A weight is 2^((S - from) cs - less). f32: from is the chunk's largest S; off is log2 of what the weights are
+            // relative to, beside ref.
+            float from[CHUNKS], less[CHUNKS], off[CHUNKS];
             if constexpr (SPLIT) {
                 // Where v is so small that its weights would be lost to the sum, they are kept, but below what counts for O.
                 const float4 e = *reinterpret_cast<const float4*>(v_exp[slot]);
                 const float es[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    mc[u] = fminf(ref + es[u], ceilf(fmaxf(t[u], kNone)) + 60.0f) - (float)kWeightExp;
+                for (int u = 0; u < 4; ++u) {
+                    const float d = fmaxf(t[u] - ref, -65536.0f);
+                    from[u] = raw[u] == -INFINITY ? 0.0f : raw[u];
+                    off[u] = fminf(off_o + es[u], ceilf(d) + 60.0f) - (float)kWeightExp, less[u] = off[u] - d;
+                }
             } else {
-                mc[0] = (ref == -INFINITY ? 0.0f : ref) * c;
+                from[0] = ref == -INFINITY ? 0.0f : ref;
             }
             uint64_t sum = 0;
             auto gather = [&](float factor) {
@@ -561,12 +570,12 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int at = g * 32 + 2 * i, u = SPLIT ? at / kChunk : 0;
+                        const uint64_t x = add2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), pair(-from[u], -from[u]));
                         float p0, p1;
-                        unpair(fma2(pair(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), pair(cs[u], cs[u]),
-                                    pair(-mc[u], -mc[u])), p0, p1);
+                        unpair(SPLIT ? fma2(x, pair(cs[u], cs[u]), pair(-less[u], -less[u])) : mul2(x, pair(c, c)), p0, p1);
                         p0 = ex2(p0), p1 = ex2(p1);
                         sum = add2(sum, pair(p0, p1));
-                        if (SPLIT && (at + 2) % kChunk == 0) gather(pow2(mc[u] + (float)kWeightExp - ref_l));
+                        if (SPLIT && (at + 2) % kChunk == 0) gather(pow2(off[u] + (float)kWeightExp));
                         if constexpr (SPLIT)
                             split2(p0, p1, hi[i], lo[i]);
                         else
@@ -609,12 +618,12 @@ __global__ void __launch_bounds__(kThreads, is_f32<OUT>() && PANELS == 2 ? 1 : 2
             // is relative to turned into what the sum is, in two steps as the power of two may leave f32's range.
             float f = a.splits > 1 ? (SPLIT ? 1.0f / (1 << kWeightExp) : 1.0f) : (l == 0.0f ? 0.0f : 1.0f / l), f2 = 1.0f;
             if constexpr (SPLIT) {
-                const float e = ref - ref_l, half = floorf(0.5f * e);
-                f *= pow2(half), f2 = pow2(e - half);
+                const float half = floorf(0.5f * off_o);
+                f *= pow2(half), f2 = pow2(off_o - half);
             }
             float* part = a.part + (at * a.splits + split) * (a.dim + 4);
             if (a.splits > 1 && store) {
-                part[a.dim] = l == 0.0f ? -INFINITY : (SPLIT ? ref_l : ref * c);
+                part[a.dim] = l == 0.0f ? -INFINITY : (SPLIT ? ref : ref * c);
                 part[a.dim + 1] = SPLIT ? l / (1 << kWeightExp) : l;
             }
             columns([&](int i) {

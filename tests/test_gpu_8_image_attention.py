@@ -709,3 +709,30 @@ def test_a_captured_layer(mbx):
             close(out.numpy(), want, tol)
         ctx.set_stream(None)
         del graph
+
+
+@pytest.mark.parametrize("heads", [2, 148])
+@pytest.mark.parametrize("nq", [2, 140])
+@pytest.mark.parametrize("kind", DTYPES)
+def test_block_attention_of_logits_beyond_a_step_of_one(mbx, ctx, kind, nq, heads):
+    """Logits of up to 2^31, where f32 numbers are far more than one apart, and all of them exact: the largest takes all."""
+    nk, dim = 640, 40
+    rng = np.random.default_rng(73)
+    steps = (np.arange(nk) * 37 % nk - 200) * (1 if kind == "bf16" else 64)  # distinct, 8 bits of bf16 at the top below
+    if kind == "bf16":
+        steps = np.where(np.abs(steps) > 255, -3, steps)
+        steps[5] = 256
+    q, k = np.zeros((1, nq, heads, dim)), np.zeros((1, nk, 1, dim))
+    q[..., 0] = 2.0 ** (15 if kind == "f16" else 20) * np.where(np.arange(nq) % 2, 1, 0.75)[None, :, None]
+    k[0, :, 0, 0] = steps
+    size = 2.0 ** rng.integers(-6, 7, nk // 16).repeat(16)  # f32: another scale every 16 keys
+    v = rng.standard_normal((1, nk, 1, dim)) * size[None, :, None, None]
+    q, k, v = (ref.narrow(t, kind) for t in (q, k, v))
+    index = np.broadcast_to(np.arange(10, dtype=np.int32), (1, heads, -(-nq // 128), 10)).copy()
+    wide = ref.wide(v)[0, :, 0]
+    for scale, best in ((1.0, steps.argmax()), (-1.0, steps.argmin())):
+        if (steps == steps[best]).sum() > 1:
+            continue
+        out = mbx.block_attention(*(up(ctx, t) for t in (q, k, v, index)), scale=scale)
+        want = np.broadcast_to(wide[best], q.shape)
+        close(out.numpy(), want, 2.0 ** -20 * np.abs(want) + ref.HALF_STEP[kind] * np.abs(want))
