@@ -42,16 +42,16 @@
 // weights is relative to that of x. Both are whole numbers, so every rescaling is exact.
 // The tensor core truncates as it adds into its f32 accumulator, so a long sum there drifts by about 2^-25 a
 // step: the softmax threads add each tile's P·V to a second set of TMEM columns, rounding to nearest, and the
-// next tile begins a fresh sum. (16 x 4096 x 8 x 40 over 1024 keys, relative to the exact result: 3.0e-7 in
-// 549 us, with sums over two tiles 5.5e-7 in 543 us; a plain f32 softmax has 5.9e-7. With 80 channels 3.0e-7
-// against 5.5e-7 and plain 5.1e-7.)
+// next tile begins a fresh sum. (16 x 4096 x 8 x 40 over 1024 keys, relative to the exact result: 3.2e-7, with
+// sums over two tiles 5.5e-7 and 1 % less time; a plain f32 softmax has 5.9e-7. With 80 channels 3.2e-7 against
+// 5.5e-7 and 7 % less time; plain 5.1e-7.)
 //
 // Masked keys: S becomes −inf; their V rows become zero in shared memory (16-bit) or while
 // splitting (f32), since zero times what a mask hides may be NaN.
 // Measured on a B200, in a burst of ten calls and in a run of two seconds, in which the card clocks down:
-// 32768 queries x 16 heads x 128 bf16 over 2048 keys each in 527 and 612 us (1043 and 898 TFLOP/s; tensor cores
-// 50 % busy, exponentials 51 %), 2 x 16384 x 16 x 64 f16 over 2048 keys in 421 and 441 us (653 and 624 TFLOP/s;
-// exponentials 61 %), 16 x 4096 x 8 x 40 f32 over 1024 keys in 494 and 548 us with the split (174 and 157 TFLOP/s,
+// 32768 queries x 16 heads x 128 bf16 over 2048 keys each in 546 and 615 us (1007 and 894 TFLOP/s; tensor cores
+// 50 % busy, exponentials 51 %), 2 x 16384 x 16 x 64 f16 over 2048 keys in 450 and 457 us (611 and 601 TFLOP/s;
+// exponentials 59 %), 16 x 4096 x 8 x 40 f32 over 1024 keys in 521 and 563 us with the split (165 and 153 TFLOP/s,
 // three times that in products).
 // Every wait is bounded; on timeout the CTA records the error, waits (bounded) for its copies and
 // MMAs in flight, frees TMEM and returns. It looks for them when every warp has stopped: a producer may be through
