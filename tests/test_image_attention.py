@@ -87,7 +87,6 @@ def test_block_select_refuses(mbx, blank, change, text):
 
 @pytest.mark.parametrize("change,text", BAD_BLOCKS + [c for c in BAD_TENSORS if "workspace" not in c[1]] + [
     (dict(dim=136, q_stride=272, k_stride=136, v_stride=136), "dim"), (dict(v_stride=24), "stride"),
-    (dict(dtype=3 | 16), "dtype"), (dict(dtype=1 | 32), "dtype"),
     (dict(v=A + 4), "aligned"), (dict(v=None), "v"), (dict(out=None), "out"), (dict(out=A + 8), "aligned"),
     (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale")])
 def test_block_attention_refuses(mbx, blank, change, text):
@@ -147,10 +146,6 @@ def test_python_front_end_refuses_mismatched_tensors(mbx):
         mbx.block_attention(q, k, k, t((1, 2, 2, 3), np.int32), workspace=q, out=q)
     with pytest.raises(ValueError, match="index"):
         mbx.block_attention(q, k, k, t((1, 2, 1, 3), np.float32), workspace=q, out=q)
-    with pytest.raises(ValueError, match="out"):
-        mbx.block_attention(q, k, k, index, workspace=q, out=t((1, 4, 2, 16), mbx.bfloat16))
-    with pytest.raises(ValueError, match="out"):
-        mbx.block_attention(q, k, k, index, workspace=q, out=t((1, 4, 2, 8), np.float32))
     with pytest.raises(ValueError, match="v must"):
         mbx.block_attention(q, k, t((1, 6, 1, 16)), index, workspace=q, out=q)
     with pytest.raises(ValueError, match="key_mask"):
@@ -198,6 +193,19 @@ def test_python_front_end_refuses_tensors_of_another_device(mbx):
                 call(**{name: other})
             with pytest.raises(mbx.MbxError, match="context"):  # past the front end: there is no handle
                 call(**{name: same})
+
+
+def test_block_attention_refuses_other_results(mbx, blank):
+    """The result is float32 or of the operands' type."""
+    for dtype in (3 | mbx.abi.OUT_F32, 1 | 32, -1):
+        _refused(mbx, _attend(mbx, blank, {**BLOCK, "dtype": dtype}), "dtype")
+
+    def t(shape, dtype=np.float16):
+        return mbx.DeviceTensor.wrap(None, A, shape, dtype=dtype)
+    q, k, index = t((1, 4, 2, 16)), t((1, 5, 1, 16)), t((1, 2, 1, 3), np.int32)
+    for out in (t((1, 4, 2, 16), mbx.bfloat16), t((1, 4, 2, 8), np.float32), t((1, 4, 2, 8))):
+        with pytest.raises(ValueError, match="out"):
+            mbx.block_attention(q, k, k, index, workspace=q, out=out)
 
 
 def test_tensor_size_is_a_plain_integer(mbx):
