@@ -24,9 +24,10 @@
 // operand as it lies, so nothing is transposed.
 //
 // 16-bit operands: P is rounded to their type: half a step of a weight, beside half a step of the
-// result at the end (2.16e-4 of the exact result at 1024 px and 1.73e-3 for video, where the result's rounding
-// alone is 2.07e-4 and 1.66e-3). Exact weights would be two parts of each, half as many tensor products again in a
-// kernel that is bound by them and by the instructions that make the weights. The weights are relative to a reference that is raised only when a row's
+// result at the end: 2.16e-4 of the exact result at 1024 px and 1.73e-3 for video, where the result's rounding
+// alone is 2.07e-4 and 1.66e-3. Weights in two parts come to that, for half as many tensor products again and more
+// instructions a weight (1024 px 573 us against 462, video 761 against 623): not worth it in types whose users
+// round more elsewhere; float32 operands have them. The weights are relative to a reference that is raised only when a row's
 // maximum outgrows it by 2^8, so O, which accumulates in TMEM over the whole list, is rarely
 // rescaled. The reference comes off S before the factor: as one fused step, its own product is rounded to a
 // step of f32, which past logits of 2^24 is more than one and past 2^27 more than f16's weights can hold
